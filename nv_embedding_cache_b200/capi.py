@@ -100,6 +100,49 @@ class ShardedLookup(C.Structure):
                 ("output_dtype", _i32)]
 
 
+# ---- paged key/value cache (include/nve_b200_kv.h) -------------------------------------------
+DTYPE_E4M3 = 4
+KV_BAD_PAGE, KV_BAD_LENGTH, KV_BAD_AXIS = 1, 2, 4
+
+
+class KvCache(C.Structure):
+    _fields_ = [("keys", _vp), ("values", _vp), ("key_strides", _i64 * 3), ("value_strides", _i64 * 3),
+                ("weights", _vp), ("key_scale", _vp), ("value_scale", _vp), ("dtype", _i32), ("num_pages", _i64),
+                ("page_size", _i32), ("num_heads", _i32), ("head_width", _i32), ("status", _vp)]
+
+
+class HeadRows(C.Structure):
+    _fields_ = [("in_", _vp), ("out", _vp), ("in_token_stride", _i64), ("in_head_stride", _i64),
+                ("out_token_stride", _i64), ("out_head_stride", _i64), ("num_heads", _i32)]
+
+
+class Rotary(C.Structure):
+    _fields_ = [("positions", _vp), ("axis_stride", _i64), ("token_stride", _i64), ("num_axes", _i32),
+                ("inv_freq", _vp), ("pair_axis", _vp), ("num_pairs", _i32), ("interleaved", _i32), ("status", _vp)]
+
+
+class KvAppend(C.Structure):
+    _fields_ = [("dtype", _i32), ("num_tokens", _i64), ("q", HeadRows), ("k", HeadRows), ("v", HeadRows),
+                ("rotary", C.POINTER(Rotary)), ("page_table", _vp), ("page_table_stride", _i64),
+                ("pages_per_sequence", _i32), ("num_sequences", _i32), ("lengths", _vp), ("csr_offsets", _vp),
+                ("new_lengths", _vp), ("zero_padding", _i32)]
+
+
+class KvAttend(C.Structure):
+    _fields_ = [("dtype", _i32), ("num_sequences", _i32), ("num_q_heads", _i32), ("q", _vp),
+                ("q_sequence_stride", _i64), ("q_head_stride", _i64), ("out", _vp), ("out_sequence_stride", _i64),
+                ("out_head_stride", _i64), ("lse", _vp), ("page_table", _vp), ("page_table_stride", _i64),
+                ("pages_per_sequence", _i32), ("lengths", _vp), ("max_length", _i32), ("scale", C.c_float),
+                ("accumulate_weights", _i32)]
+
+
+class KvEvict(C.Structure):
+    _fields_ = [("num_sequences", _i32), ("page_table", _vp), ("page_table_stride", _i64),
+                ("pages_per_sequence", _i32), ("lengths", _vp), ("max_length", _i32), ("new_page_table", _vp),
+                ("new_page_table_stride", _i64), ("new_pages_per_sequence", _i32), ("budget", _i32), ("sinks", _i32),
+                ("recent", _i32), ("kept", _vp), ("new_lengths", _vp)]
+
+
 class NveError(RuntimeError):
     def __init__(self, status: int, message: str):
         super().__init__(f"nve status {status}: {message}")
@@ -214,6 +257,11 @@ PROTOTYPES = {
     "nve_b200_scatter_rows": (_i32, [_vp, _i64, _vp, _i64, _i64, _vp, _i64, _vp]),
     "nve_b200_managed_block_create": (_i32, [C.POINTER(_vp), _u64, C.POINTER(_i32), _i32]),
     "nve_b200_managed_block_destroy": (_i32, [_vp]),
+    # paged key/value cache (include/nve_b200_kv.h)
+    "nve_b200_rotary": (_i32, [C.POINTER(Rotary), _i32, _i32, _i64, C.POINTER(HeadRows), _i32, _i32, _vp]),
+    "nve_b200_kv_append": (_i32, [C.POINTER(KvCache), C.POINTER(KvAppend), _vp]),
+    "nve_b200_kv_attend": (_i32, [C.POINTER(KvCache), C.POINTER(KvAttend), _vp, C.POINTER(C.c_size_t), _vp]),
+    "nve_b200_kv_evict": (_i32, [C.POINTER(KvCache), C.POINTER(KvEvict), _vp]),
 }
 
 for _name, (_res, _args) in PROTOTYPES.items():

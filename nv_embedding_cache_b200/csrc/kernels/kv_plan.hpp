@@ -1,0 +1,58 @@
+// Arithmetic the kernels of the paged cache and their host code share, plain C++ so that it can be checked without a
+// GPU: division by an invariant, and the cut of the attention's tiles into runs.
+#pragma once
+
+#include <cstdint>
+
+#ifdef __CUDACC__
+#define NVE_KV_FN __host__ __device__ __forceinline__
+#else
+#define NVE_KV_FN inline
+#endif
+
+namespace nve_b200 {
+
+// n / d for 0 <= n < 2^31, 1 <= d < 2^31, by one multiply: magic = ceil(2^(31 + l) / d), l = ceil(log2 d), is below
+// 2^32 and at most 2^(31 + l) / d + 1, and the error n / 2^(31 + l) that this 1 brings stays below 1 / d
+// (Granlund and Montgomery 1994).
+struct FastDiv {
+  uint32_t d, magic, shift;
+};
+inline FastDiv make_fast_div(uint32_t d) {
+  FastDiv f{d, 0, 0};
+  if (d <= 1) return f;
+  uint32_t l = 0;
+  while ((uint64_t{1} << l) < d) l++;
+  f.shift = l - 1;
+  f.magic = static_cast<uint32_t>(((uint64_t{1} << (31 + l)) + d - 1) / d);
+  return f;
+}
+NVE_KV_FN uint32_t fast_div(uint32_t n, const FastDiv& f) {
+  return f.d <= 1 ? n : static_cast<uint32_t>((static_cast<uint64_t>(n) * f.magic) >> 32) >> f.shift;
+}
+
+// ---- tiles of the attention -----------------------------------------------------------------------
+// Tiles (64 rows of one unit = a key head and a chunk of its query heads) are numbered sequence by sequence, inside
+// a sequence unit by unit, inside a unit along the length.  CTA c of n takes the run [c total / n, (c + 1) total / n):
+// every CTA gets the same number of tiles, give or take one, whatever the lengths are.  n <= total, so no run is empty.
+constexpr int kKvTile = 64;
+
+NVE_KV_FN int32_t tiles_of(int32_t length) {
+  return static_cast<int32_t>((static_cast<int64_t>(length) + kKvTile - 1) / kKvTile);
+}
+
+struct TileRange {
+  int32_t first, last;
+};
+NVE_KV_FN TileRange tile_range(int64_t total, int32_t n, int32_t c) {
+  return {static_cast<int32_t>(total * c / n), static_cast<int32_t>(total * (c + 1) / n)};
+}
+// The CTA whose run holds tile t: the largest c with c total < (t + 1) n.
+NVE_KV_FN int32_t cta_of_tile(int64_t total, int32_t n, int32_t t) {
+  return static_cast<int32_t>(((static_cast<int64_t>(t) + 1) * n - 1) / total);
+}
+// A CTA leaves at most two unfinished units: the one its run begins in and the one it ends in.  Slot of the unit that
+// begins at tile `unit_first` in the scratch of a CTA whose run begins at `run_first`.
+NVE_KV_FN int32_t part_slot(int32_t run_first, int32_t unit_first) { return run_first >= unit_first ? 0 : 1; }
+
+}  // namespace nve_b200

@@ -1,0 +1,16 @@
+// The host arithmetic of the paged cache (csrc/kernels/kv_plan.hpp) for tests without a GPU.
+#include "kernels/kv_plan.hpp"
+
+using namespace nve_b200;
+
+extern "C" {
+uint32_t kp_div(uint32_t n, uint32_t d) { return fast_div(n, make_fast_div(d)); }
+int32_t kp_tiles(int32_t length) { return tiles_of(length); }
+void kp_range(int64_t total, int32_t n, int32_t c, int32_t* out) {
+  const TileRange r = tile_range(total, n, c);
+  out[0] = r.first;
+  out[1] = r.last;
+}
+int32_t kp_cta(int64_t total, int32_t n, int32_t t) { return cta_of_tile(total, n, t); }
+int32_t kp_slot(int32_t run_first, int32_t unit_first) { return part_slot(run_first, unit_first); }
+}
