@@ -34,7 +34,8 @@ extern "C" {
 enum {
   NVE_B200_KV_BAD_PAGE = 1,   /* a page id outside [0, num_pages): the row was left out */
   NVE_B200_KV_BAD_LENGTH = 2, /* a length below 0 or above the capacity: clamped; an appended row without a place */
-  NVE_B200_KV_BAD_AXIS = 4    /* a pair_axis outside [0, num_axes): the pair was not turned */
+  NVE_B200_KV_BAD_AXIS = 4,   /* a pair_axis outside [0, num_axes): the pair was not turned */
+  NVE_B200_KV_TIMED_OUT = 8   /* a wait inside a kernel ran into its limit: the outputs of that call are not complete */
 };
 
 /* A paged cache.  Rows are head_width values of one head of one token; the last dimension is dense. */

@@ -102,7 +102,7 @@ class ShardedLookup(C.Structure):
 
 # ---- paged key/value cache (include/nve_b200_kv.h) -------------------------------------------
 DTYPE_E4M3 = 4
-KV_BAD_PAGE, KV_BAD_LENGTH, KV_BAD_AXIS = 1, 2, 4
+KV_BAD_PAGE, KV_BAD_LENGTH, KV_BAD_AXIS, KV_TIMED_OUT = 1, 2, 4, 8
 
 
 class KvCache(C.Structure):

@@ -229,8 +229,11 @@ void attend(const nve_b200_kv_cache_t* cache, const nve_b200_kv_attend_t* a, voi
   p.chunk = static_cast<int32_t>(ceil_div(p.group, p.chunks));
   p.rows_per_unit = p.chunk <= 16 ? 16 : (p.chunk <= 32 ? 32 : 64);
   const int64_t units = static_cast<int64_t>(cache->num_heads) * p.chunks;
-  const int64_t tiles = a->num_sequences * units * ceil_div(p.table.capacity, kKvTile);
-  NVE_B200_ARG(tiles < kIntMax && static_cast<int64_t>(a->num_sequences) * p.q_heads < kIntMax, who,
+  p.tile_rows = kv_tile_rows(cache->head_width, static_cast<int>(value_bytes(cache->dtype)));
+  const int64_t tiles = a->num_sequences * units * ceil_div(p.table.capacity, p.tile_rows);
+  NVE_B200_ARG(tiles < kIntMax && static_cast<int64_t>(a->num_sequences) * p.q_heads < (1 << 30) &&
+                   static_cast<int64_t>(a->num_sequences) * cache->num_heads * ceil_div(p.table.capacity, 1024) < (1 << 30),
+               who,
                ": too many rows for one call");
   if (a->num_sequences == 0) {
     if (scratch == nullptr) *scratch_bytes = 0;
@@ -245,7 +248,7 @@ void attend(const nve_b200_kv_cache_t* cache, const nve_b200_kv_attend_t* a, voi
   p.part_ml = carve<float2>(at, part_rows);
   if (a->accumulate_weights) {
     p.unit_lse = carve<float>(at, a->num_sequences * units * p.rows_per_unit);
-    p.scores = carve<float>(at, std::max<int64_t>(tiles, 1) * p.chunk * kKvTile);
+    p.scores = carve<float>(at, std::max<int64_t>(tiles, 1) * p.chunk * p.tile_rows);
   }
   const size_t need = static_cast<size_t>(at - begin);
   if (scratch == nullptr) {
@@ -269,7 +272,7 @@ void attend(const nve_b200_kv_cache_t* cache, const nve_b200_kv_attend_t* a, voi
   p.q_bf16 = a->dtype == NVE_DTYPE_BFLOAT16;
   p.scale_log2 = a->scale * 1.44269504088896340736f;
   launch_kv_attend(p, cache->dtype, stream);
-  launch_kv_join(p, sm_count(), stream);
+  launch_kv_join(p, stream);
 }
 
 void evict(const nve_b200_kv_cache_t* cache, const nve_b200_kv_evict_t* a, cudaStream_t stream) {

@@ -6,17 +6,18 @@
 // What bounds it: 2 width values are read per (row, key head) and 4 width flops done per query head of the group, so
 // even 16 query heads on one key head ask for a few per cent of the tensor rate: memory does.  Everything here is
 // there to keep loads in flight on every SM, whatever the batch looks like:
-//  * the tiles (64 rows of one key head) of the whole batch are one list, cut into equal runs, one per resident CTA
+//  * the tiles (64 or 128 rows of one key head) of the whole batch are one list, cut into equal runs, one per resident CTA
 //    (kv_plan.hpp): one long sequence and a ragged batch load all SMs alike.  A unit that falls into several
 //    runs leaves (m, sum, weighted sum) per run in scratch and is joined by kv_join.cu.
-//  * a CTA's tiles are one stream through a ring of shared-memory stages filled by cp.async (16 bytes each, a
-//    page may end anywhere in a tile); the ring runs on across units, the queries of a unit travel with its
-//    first tile.
+//  * a CTA's tiles are one stream through a ring of shared-memory stages.  Two warps do nothing but look rows up in
+//    the page table and fill the ring with cp.async (16 bytes each: a page may end anywhere in a tile, rows have
+//    any strides), four warps compute; full and empty barriers per stage, no barrier over all warps.  The ring
+//    runs on across units, the queries of a unit travel with its first tile.
 //  * mma.sync m16n8k16, not tcgen05: a tile has as few as one query row, a 128-row tcgen05 tile would be 8 to
 //    128 times padding and its accumulator would have to leave TMEM for the running maximum every 64 rows.  Here
 //    the scores stay in the registers that the second product takes them from.
-// Four warps; with up to 16 query heads each warp takes 16 rows of the tile and its own running maximum, and
-// the four are joined when the unit ends; with more, warps take 16 heads each and share the rows.
+// With up to 16 query heads each of the four warps takes a quarter of the tile's rows and has its own running maximum,
+// and the four are joined when the unit ends; with more, warps take 16 heads each and share the rows.
 //
 // Probabilities are rounded to the type of the values (f16 for E4M3 rows: exact for them, see below) before the
 // second product: relative 2^-9 (bf16) or 2^-12 of each, below the rounding of the output; the sum is taken before that.
@@ -34,17 +35,23 @@ namespace nve_b200 {
 
 namespace kv {
 
-constexpr int kThreads = 128;
+constexpr int kComputeWarps = 4;
+constexpr int kLoadWarps = 2;
+constexpr int kThreads = (kComputeWarps + kLoadWarps) * 32;
 constexpr float kNegInf = -__builtin_huge_valf();
 
 __device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, bool take) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(take ? 16 : 0) : "memory");
 }
-__device__ __forceinline__ void cp_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-template <int N>
-__device__ __forceinline__ void cp_wait() {
-  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+// The barrier gets this thread's arrival when its copies so far are done.
+__device__ __forceinline__ void cp_async_arrive(uint64_t* bar) {
+  asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(smem_addr(bar)) : "memory");
 }
+__device__ __forceinline__ void cp_async_wait_all() { asm volatile("cp.async.wait_all;" ::: "memory"); }
+__device__ __forceinline__ void mbar_arrive(uint64_t* bar) {
+  asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_addr(bar)) : "memory");
+}
+__device__ __forceinline__ void compute_sync() { asm volatile("bar.sync 1, %0;" ::"n"(kComputeWarps * 32) : "memory"); }
 __device__ __forceinline__ void ldsm4(uint32_t (&r)[4], uint32_t addr) {
   asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
                : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
@@ -80,13 +87,11 @@ __device__ __forceinline__ float exp2_fast(float x) {
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
-// two E4M3 values (bits 0-15) as f16x2; exact
-__device__ __forceinline__ uint32_t e4m3_to_f16(uint32_t two) {
-  const __half2_raw h = __nv_cvt_fp8x2_to_halfraw2(static_cast<__nv_fp8x2_storage_t>(two & 0xffffu), __NV_E4M3);
-  return static_cast<uint32_t>(h.x) | (static_cast<uint32_t>(h.y) << 16);
-}
-__device__ __forceinline__ float to_float(const uint8_t* p, bool bf16) {
-  return bf16 ? __bfloat162float(*reinterpret_cast<const __nv_bfloat16*>(p)) : __half2float(*reinterpret_cast<const __half*>(p));
+// four E4M3 values as two f16x2; exact
+__device__ __forceinline__ void e4m3_to_f16(uint32_t four, uint32_t& lo, uint32_t& hi) {
+  asm("{\n\t.reg .b16 a, b;\n\tmov.b32 {a, b}, %2;\n\t"
+      "cvt.rn.f16x2.e4m3x2 %0, a;\n\tcvt.rn.f16x2.e4m3x2 %1, b;\n\t}"
+      : "=r"(lo), "=r"(hi) : "r"(four));
 }
 __device__ __forceinline__ void store16(uint8_t* p, float x, bool bf16) {
   if (bf16) *reinterpret_cast<__nv_bfloat16*>(p) = __float2bfloat16_rn(x);
@@ -107,23 +112,23 @@ struct Shape {
   static constexpr bool kE4m3 = sizeof(ST) == 1;
   static constexpr int kRowBytes = DP * sizeof(ST);
   static constexpr int kChunks = kRowBytes / 16;          // 16-byte chunks of a row
-  static constexpr int kTileBytes = kKvTile * kRowBytes;  // keys or values of a tile
-  static constexpr int kWT = 4 / WM;                      // warps along the rows
-  static constexpr int kWarpRows = kKvTile / kWT;         // rows of a tile one warp takes
+  static constexpr int kTile = kv_tile_rows(DP, sizeof(ST));
+  static constexpr int kTileBytes = kTile * kRowBytes;    // keys or values of a tile
+  static constexpr int kWT = kComputeWarps / WM;          // warps along the rows
+  static constexpr int kWarpRows = kTile / kWT;           // rows of a tile one warp takes
   static constexpr int kUnitRows = 16 * WM;               // query rows
   static constexpr int kQBytes = kUnitRows * DP * 2;
-  // A stage holds a tile and the queries of the unit that may begin with it.  Stages until an SM holds three CTAs of
-  // three or more, else two, else one: 100 to 150 KB in flight per SM either way, which is what the memory's latency
-  // times its rate asks for (about 45 KB), with room for the CTA that is between two waits.
+  // A stage holds a tile and the queries of the unit that may begin with it.  Two CTAs per SM of three or more stages
+  // where they fit, else one: 130 KB and more in flight per SM; the memory's latency times its rate asks for 45 KB.
   static constexpr int kStageBytes = 2 * kTileBytes + kQBytes;
-  static constexpr int kStages = 3 * kStageBytes <= 72000 ? (73000 / kStageBytes < 6 ? 73000 / kStageBytes : 6)
-                                 : 3 * kStageBytes <= 111000 ? 3
-                                 : (222000 / kStageBytes < 5 ? 222000 / kStageBytes : 5);
-  static constexpr int kMinCtas = 3 * kStageBytes <= 72000 ? 3 : (3 * kStageBytes <= 111000 ? 2 : 1);
-  static constexpr int kMasks = 8;                        // ring of row masks, longer than the ring of stages
-  static constexpr int kOffsBytes = 2 * kKvTile * 16;
-  static constexpr int kSmem = kStages * kStageBytes + kOffsBytes + 4 * 16 * 8 + kMasks * 8 + kUnitRows * 4;
-  static_assert(kStages >= 2 && kStages < kMasks, "stages");
+  static constexpr int kMinCtas = 3 * kStageBytes <= 111000 ? 2 : 1;
+  static constexpr int kStages = kMinCtas == 2 ? (111000 / kStageBytes < 5 ? 111000 / kStageBytes : 5)
+                                               : (222000 / kStageBytes < 5 ? 222000 / kStageBytes : 5);
+  static constexpr int kMaskWords = kTile / 32;
+  static constexpr int kOffsBytes = kTile * 16;
+  static constexpr int kSmem = kStages * kStageBytes + kOffsBytes + kComputeWarps * 16 * 8 + kStages * kMaskWords * 4 +
+                               kUnitRows * 4 + kStages * 16 + 16;
+  static_assert(kStages >= 2, "stages");
 };
 
 // Byte offset of 16-byte chunk c of row r: chunks of 128 bytes are permuted by the row, so that the eight rows one
@@ -144,29 +149,38 @@ __global__ void __launch_bounds__(kThreads, Shape<ST, DP, WM>::kMinCtas) attend_
   constexpr bool kKeepQ = DP <= 128;                       // the queries stay in registers; wider ones in shared memory
   extern __shared__ __align__(1024) uint8_t smem[];
   uint8_t* const qbuf = smem + S::kStages * 2 * S::kTileBytes;
-  longlong2* const offs = reinterpret_cast<longlong2*>(qbuf + S::kStages * S::kQBytes);             // [2][kKvTile]
-  float2* const ml = reinterpret_cast<float2*>(reinterpret_cast<uint8_t*>(offs) + S::kOffsBytes);   // [4][16]
-  uint32_t* const masks = reinterpret_cast<uint32_t*>(ml + 4 * 16);                                 // [kMasks][2]
-  float* const q_up = reinterpret_cast<float*>(masks + S::kMasks * 2);                              // [kUnitRows]
+  longlong2* const offs = reinterpret_cast<longlong2*>(qbuf + S::kStages * S::kQBytes);             // [kTile]
+  uint64_t* const full = reinterpret_cast<uint64_t*>(reinterpret_cast<uint8_t*>(offs) + S::kOffsBytes);   // [kStages]
+  uint64_t* const empty = full + S::kStages;                                                        // [kStages]
+  float2* const ml = reinterpret_cast<float2*>(empty + S::kStages);                                 // [warps][16]
+  uint32_t* const masks = reinterpret_cast<uint32_t*>(ml + kComputeWarps * 16);                     // [kStages][kMaskWords]
+  float* const q_up = reinterpret_cast<float*>(masks + S::kStages * S::kMaskWords);                 // [kUnitRows]
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-  const int wm = warp % WM, wt = warp / WM;                // heads 16 wm.., rows kWarpRows wt.. of the tile
   const int width = p.cache.width;
-  const int row_chunks = width * static_cast<int>(sizeof(ST)) / 16;
-  const int q_chunks = width / 8;
   const int units = p.cache.heads * p.chunks;
 
+  if (tid == 0) {
+    for (int s = 0; s < S::kStages; s++) {
+      // every loading thread's copies, and each loading warp's word on which rows are there
+      mbar_init(full + s, kLoadWarps * 32 + kLoadWarps);
+      mbar_init(empty + s, kComputeWarps);
+    }
+  }
   // ---- the number of tiles, and where this CTA's run of them begins
-  __shared__ int64_t s_sum[4];
+  __shared__ int64_t s_sum[kThreads / 32];
   __shared__ int32_t s_start[3];
   {
     int64_t mine = 0;
-    for (int b = tid; b < p.table.sequences; b += kThreads) mine += tiles_of(kv_length(p.table, b, p.cache.status));
+    for (int b = tid; b < p.table.sequences; b += kThreads) mine += tiles_of(kv_length(p.table, b, p.cache.status), S::kTile);
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) mine += __shfl_xor_sync(0xffffffffu, mine, o);
     if (lane == 0) s_sum[warp] = mine;
     __syncthreads();
   }
-  const int64_t total = (s_sum[0] + s_sum[1] + s_sum[2] + s_sum[3]) * units;
+  int64_t total = 0;
+#pragma unroll
+  for (int w = 0; w < kThreads / 32; w++) total += s_sum[w];
+  total *= units;
   // no tile names a sequence without rows
   for (int b = blockIdx.x; b < p.table.sequences; b += gridDim.x) {
     if (kv_length(p.table, b, nullptr) == 0) {
@@ -189,7 +203,7 @@ __global__ void __launch_bounds__(kThreads, Shape<ST, DP, WM>::kMinCtas) attend_
     int64_t before = 0;
     for (int base = 0; base < p.table.sequences; base += 32) {
       const int b = base + lane;
-      const int nt = b < p.table.sequences ? tiles_of(kv_length(p.table, b, nullptr)) : 0;
+      const int nt = b < p.table.sequences ? tiles_of(kv_length(p.table, b, nullptr), S::kTile) : 0;
       const int64_t here = static_cast<int64_t>(nt) * units;
       int64_t incl = here;
 #pragma unroll
@@ -209,101 +223,117 @@ __global__ void __launch_bounds__(kThreads, Shape<ST, DP, WM>::kMinCtas) attend_
     }
   }
   __syncthreads();
-  TileCursor take;                                          // the tile whose rows are located next
-  take.b = s_start[0];
-  take.unit = s_start[1];
-  take.j = s_start[2];
-  take.length = kv_length(p.table, take.b, nullptr);
-  take.tiles = tiles_of(take.length);
-  TileCursor issue = take, use = take;                      // the tile whose copies are issued next; the tile in use
+  TileCursor at;
+  at.b = s_start[0];
+  at.unit = s_start[1];
+  at.j = s_start[2];
+  at.length = kv_length(p.table, at.b, nullptr);
+  at.tiles = tiles_of(at.length, S::kTile);
+  int stage = 0;
+  uint32_t phase = 0;                                       // of the stage's barriers
 
-  // Offsets of the row of the `take` tile this thread (tid < kKvTile) looks after; negative: no such row.
-  auto locate = [&]() -> longlong2 {
-    const int32_t row = take.j * kKvTile + tid;
-    longlong2 o = make_longlong2(-1, -1);
-    if (row < take.length) {
-      int32_t slot;
-      const int32_t page = kv_locate(p.cache, p.table.pages, p.table.stride, take.b, row, &slot);
-      const int32_t head = take.unit / p.chunks;
-      if (page >= 0) {
-        o.x = page * p.cache.k_page + slot * p.cache.k_slot + head * p.cache.k_head;
-        o.y = page * p.cache.v_page + slot * p.cache.v_slot + head * p.cache.v_head;
-      }
-    }
-    return o;
-  };
-  auto keep_located = [&](int i, longlong2 o) {             // warps 0 and 1, tile number i of this CTA
-    offs[(i & 1) * kKvTile + tid] = o;
-    const uint32_t mask = __ballot_sync(0xffffffffu, o.x >= 0);
-    if (lane == 0) masks[(i % S::kMasks) * 2 + warp] = mask;
-  };
-  int q_issue = 0, q_use = 0;                               // buffers of the units the two cursors are in
-  auto issue_tile = [&](int i) {                            // copies of tile number i into its stage
-    const uint32_t k_addr = smem_addr(smem) + (i % S::kStages) * 2 * S::kTileBytes, v_addr = k_addr + S::kTileBytes;
-    const longlong2* const o = offs + (i & 1) * kKvTile;
+  // the join may be scheduled from here on; it waits for this grid's end before it reads what is written here
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+
+  if (warp >= kComputeWarps) {
+    // ================================ loading warps ================================
+    constexpr int kOwnRows = S::kTile / kLoadWarps;         // rows of a tile this warp looks after
+    constexpr int kEach = kOwnRows / 32;
+    const int lw = warp - kComputeWarps;
+    const int row_chunks = width * static_cast<int>(sizeof(ST)) / 16, q_chunks = width / 8;
+    longlong2* const own = offs + lw * kOwnRows;
+    // byte offsets of this lane's rows of the tile `at`; negative: no such row
+    auto locate = [&](longlong2 (&o)[kEach]) {
+      const int32_t head = at.unit / p.chunks;
 #pragma unroll
-    for (int x = 0; x < kKvTile * S::kChunks / kThreads; x++) {
-      const int id = x * kThreads + tid;
-      const int r = id / S::kChunks, c = id % S::kChunks;
-      const longlong2 at = o[r];
-      // chunks behind the row's width and rows that are not there become zeros: a NaN left in a page never meets
-      // the products
-      const bool ok = at.x >= 0 && c < row_chunks;
-      const uint32_t to = chunk_at<S::kRowBytes>(r, c);
-      cp_async16(k_addr + to, ok ? p.cache.keys + at.x + c * 16 : p.cache.keys, ok);
-      cp_async16(v_addr + to, ok ? p.cache.values + at.y + c * 16 : p.cache.values, ok);
-    }
-    if (i == 0 || issue.j == 0) {                           // the unit's queries
-      if (i > 0) q_issue = q_issue + 1 == S::kStages ? 0 : q_issue + 1;
-      const uint32_t q_addr = smem_addr(qbuf) + q_issue * S::kQBytes;
-      const int head = issue.unit / p.chunks, first = (issue.unit % p.chunks) * p.chunk;
-      const int n = min(p.chunk, p.group - first);
-      const uint8_t* const src = p.q + issue.b * p.q_seq + (head * p.group + first) * p.q_head;
-      for (int id = tid; id < S::kUnitRows * (DP / 8); id += kThreads) {
-        const int r = id / (DP / 8), c = id % (DP / 8);
-        const bool ok = r < n && c < q_chunks;
-        cp_async16(q_addr + chunk_at<DP * 2>(r, c), ok ? src + r * p.q_head + c * 16 : p.q, ok);
+      for (int x = 0; x < kEach; x++) {
+        const int32_t row = at.j * S::kTile + lw * kOwnRows + x * 32 + lane;
+        o[x] = make_longlong2(-1, -1);
+        if (row < at.length) {
+          int32_t slot;
+          const int32_t page = kv_locate(p.cache, p.table.pages, p.table.stride, at.b, row, &slot);
+          if (page >= 0) {
+            o[x].x = page * p.cache.k_page + slot * p.cache.k_slot + head * p.cache.k_head;
+            o[x].y = page * p.cache.v_page + slot * p.cache.v_slot + head * p.cache.v_head;
+          }
+        }
       }
-    }
-    issue.advance(p.table, units);
-  };
-
-  // ---- fill the ring; rows are located one tile ahead of their copies
-  if (tid < kKvTile) keep_located(0, locate());
-  take.advance(p.table, units);
+    };
+    longlong2 next[kEach];
+    locate(next);
+    int q_at = 0;                                           // buffer of the unit's queries
 #pragma unroll 1
-  for (int i = 0; i < S::kStages - 1; i++) {
-    __syncthreads();
-    if (i < n_tiles) issue_tile(i);
-    cp_commit();
-    if (i + 1 < n_tiles) {
-      if (tid < kKvTile) keep_located(i + 1, locate());
-      take.advance(p.table, units);
+    for (int i = 0; i < n_tiles; i++) {
+      if (!mbar_wait_bounded(empty + stage, phase ^ 1)) {   // the first round passes at once
+        kv_flag(p.cache.status, NVE_B200_KV_TIMED_OUT);
+        break;
+      }
+      __syncwarp();
+#pragma unroll
+      for (int x = 0; x < kEach; x++) {
+        own[x * 32 + lane] = next[x];
+        const uint32_t mask = __ballot_sync(0xffffffffu, next[x].x >= 0);
+        if (lane == 0) masks[stage * S::kMaskWords + lw * kEach + x] = mask;
+      }
+      __syncwarp();
+      if (lane == 0) mbar_arrive(full + stage);
+      const bool first = i == 0 || at.j == 0;
+      const TileCursor now = at;
+      at.advance(p.table, units, S::kTile);
+      if (i + 1 < n_tiles) locate(next);                    // its page ids arrive while this tile's copies are issued
+      const uint32_t k_addr = smem_addr(smem) + stage * 2 * S::kTileBytes, v_addr = k_addr + S::kTileBytes;
+#pragma unroll 8
+      for (int x = 0; x < kOwnRows * S::kChunks / 32; x++) {
+        const int id = x * 32 + lane;
+        const int r = id / S::kChunks, c = id % S::kChunks;
+        const longlong2 o = own[r];
+        // chunks behind the row's width and rows that are not there become zeros: a NaN left in a page never meets
+        // the products
+        const bool ok = o.x >= 0 && c < row_chunks;
+        const uint32_t to = chunk_at<S::kRowBytes>(lw * kOwnRows + r, c);
+        cp_async16(k_addr + to, p.cache.keys + (ok ? o.x + c * 16 : 0), ok);
+        cp_async16(v_addr + to, p.cache.values + (ok ? o.y + c * 16 : 0), ok);
+      }
+      if (first) {                                          // the unit's queries
+        if (i > 0) q_at = q_at + 1 == S::kStages ? 0 : q_at + 1;
+        const uint32_t q_addr = smem_addr(qbuf) + q_at * S::kQBytes;
+        const int head = now.unit / p.chunks, q_first = (now.unit % p.chunks) * p.chunk;
+        const int n = min(p.chunk, p.group - q_first);
+        const uint8_t* const src = p.q + now.b * p.q_seq + (head * p.group + q_first) * p.q_head;
+        for (int id = lw * 32 + lane; id < S::kUnitRows * (DP / 8); id += kLoadWarps * 32) {
+          const int r = id / (DP / 8), c = id % (DP / 8);
+          const bool ok = r < n && c < q_chunks;
+          cp_async16(q_addr + chunk_at<DP * 2>(r, c), ok ? src + r * p.q_head + c * 16 : p.q, ok);
+        }
+      }
+      cp_async_arrive(full + stage);
+      if (++stage == S::kStages) {
+        stage = 0;
+        phase ^= 1;
+      }
+      __syncwarp();
     }
+    cp_async_wait_all();
+    return;
   }
 
+  // ================================ computing warps ================================
+  const int wm = warp % WM, wt = warp / WM;                 // heads 16 wm.., rows kWarpRows wt.. of the tile
   float acc[kSteps][2][4];
   float m_run[2], l_run[2];
   uint32_t qf[kKeepQ ? kSteps : 1][4];
   float row_scale[2];
   bool from_start = false;                                  // this CTA has the current unit from its first tile
+  int q_use = 0;
 
 #pragma unroll 1
   for (int i = 0; i < n_tiles; i++) {
-    cp_wait<S::kStages - 2>();
-    __syncthreads();
-    const int ahead = i + S::kStages - 1;
-    if (ahead < n_tiles) issue_tile(ahead);
-    cp_commit();
-    const bool locates = ahead + 1 < n_tiles;
-    longlong2 next = make_longlong2(-1, -1);
-    if (locates) {
-      if (tid < kKvTile) next = locate();
-      take.advance(p.table, units);
+    if (!mbar_wait_bounded(full + stage, phase)) {          // all four warps wait for the same event: all give up
+      kv_flag(p.cache.status, NVE_B200_KV_TIMED_OUT);
+      return;
     }
-
-    const int head = use.unit / p.chunks;
-    const int unit_first = (use.unit % p.chunks) * p.chunk; // first query head of the unit inside its group
+    const int head = at.unit / p.chunks;
+    const int unit_first = (at.unit % p.chunks) * p.chunk;  // first query head of the unit inside its group
     const int unit_heads = min(p.chunk, p.group - unit_first);
     const bool lower = wm * 16 < unit_heads, upper = wm * 16 + 8 < unit_heads;   // rows 0-7, 8-15 hold heads
     auto load_q = [&](int step, uint32_t (&a)[4]) {
@@ -321,9 +351,9 @@ __global__ void __launch_bounds__(kThreads, Shape<ST, DP, WM>::kMinCtas) attend_
         }
       }
     };
-    if (i == 0 || use.j == 0) {
+    if (i == 0 || at.j == 0) {
       if (i > 0) q_use = q_use + 1 == S::kStages ? 0 : q_use + 1;
-      from_start = use.j == 0;
+      from_start = at.j == 0;
 #pragma unroll
       for (int s = 0; s < kSteps; s++)
 #pragma unroll
@@ -335,7 +365,7 @@ __global__ void __launch_bounds__(kThreads, Shape<ST, DP, WM>::kMinCtas) attend_
         // Queries meet E4M3 rows as f16.  bf16 ones are brought into its range row by row: divided by the power of
         // two of the row's largest value, which the scores get back; exact but for values 2^-24 below that.
         if (p.q_bf16) {
-          for (int r = warp; r < S::kUnitRows; r += 4) {
+          for (int r = warp; r < S::kUnitRows; r += kComputeWarps) {
             uint32_t* const row = reinterpret_cast<uint32_t*>(qbuf + q_use * S::kQBytes) + r * (DP / 2);
             float2 v[DP / 64];
             uint32_t top = 0;
@@ -354,7 +384,7 @@ __global__ void __launch_bounds__(kThreads, Shape<ST, DP, WM>::kMinCtas) attend_
             for (int x = 0; x < DP / 64; x++) row[x * 32 + lane] = pack2<false>(v[x].x * down, v[x].y * down);
             if (lane == 0) q_up[r] = __uint_as_float(top << 23);
           }
-          __syncthreads();
+          compute_sync();
           row_scale[0] *= q_up[wm * 16 + (lane >> 2)];
           row_scale[1] *= q_up[wm * 16 + (lane >> 2) + 8];
         }
@@ -370,20 +400,27 @@ __global__ void __launch_bounds__(kThreads, Shape<ST, DP, WM>::kMinCtas) attend_
       }
     }
 
-    const uint32_t k_addr = smem_addr(smem) + (i % S::kStages) * 2 * S::kTileBytes, v_addr = k_addr + S::kTileBytes;
-    const int left = use.length - use.j * kKvTile;          // rows of the tile that exist
+    const uint32_t k_addr = smem_addr(smem) + stage * 2 * S::kTileBytes, v_addr = k_addr + S::kTileBytes;
+    const int left = at.length - at.j * S::kTile;           // rows of the tile that exist
+    const int w0 = wt * S::kWarpRows;
 
+    if (w0 < left && lower) {                               // uniform in the warp
+      // ---- scores of 16 heads x kWarpRows rows; one block alone is added up in two halves, so that the products
+      // do not wait for one another
+      constexpr int kSets = kBlocks == 1 ? 2 : 1;
+      float sc[kBlocks][2][4];
+      float more[2][4];
 #pragma unroll
-    for (int blk = 0; blk < kBlocks; blk++) {
-      const int r0 = wt * S::kWarpRows + blk * 16;
-      if (r0 >= left || !lower) break;                      // uniform in the warp
-      // ---- scores of 16 heads x 16 rows
-      float sc[2][4] = {};
+      for (int n = 0; n < 2; n++)
+#pragma unroll
+        for (int e = 0; e < 4; e++) {
+          more[n][e] = 0.0f;
+#pragma unroll
+          for (int blk = 0; blk < kBlocks; blk++) sc[blk][n][e] = 0.0f;
+        }
       if constexpr (!kE4m3) {
 #pragma unroll
         for (int s = 0; s < kSteps; s++) {
-          uint32_t kf[4];   // rows 0-7: columns 0-7, 8-15 of the step; rows 8-15: the same
-          ldsm4(kf, k_addr + chunk_at<S::kRowBytes>(r0 + (lane & 7) + ((lane >> 4) << 3), s * 2 + ((lane >> 3) & 1)));
           uint32_t a[4];
           if constexpr (kKeepQ) {
 #pragma unroll
@@ -391,58 +428,81 @@ __global__ void __launch_bounds__(kThreads, Shape<ST, DP, WM>::kMinCtas) attend_
           } else {
             load_q(s, a);
           }
-          mma16816<kBf16>(sc[0], a, kf[0], kf[1]);
-          mma16816<kBf16>(sc[1], a, kf[2], kf[3]);
+#pragma unroll
+          for (int blk = 0; blk < kBlocks; blk++) {
+            uint32_t kf[4];   // rows 0-7: columns 0-7, 8-15 of the step; rows 8-15: the same
+            ldsm4(kf, k_addr + chunk_at<S::kRowBytes>(w0 + blk * 16 + (lane & 7) + ((lane >> 4) << 3), s * 2 + ((lane >> 3) & 1)));
+            if (kSets == 2 && (s & 1)) {
+              mma16816<kBf16>(more[0], a, kf[0], kf[1]);
+              mma16816<kBf16>(more[1], a, kf[2], kf[3]);
+            } else {
+              mma16816<kBf16>(sc[blk][0], a, kf[0], kf[1]);
+              mma16816<kBf16>(sc[blk][1], a, kf[2], kf[3]);
+            }
+          }
         }
       } else {
 #pragma unroll
         for (int s = 0; s < kSteps; s += 2) {
-          // a 16-byte chunk is 16 values of a row, one step; a lane gets values 4 (lane & 3) to 4 (lane & 3) + 3
-          uint32_t kf[4];   // rows 0-7, 8-15 of step s; the same of step s + 1
-          ldsm4(kf, k_addr + chunk_at<S::kRowBytes>(r0 + (lane & 7) + (((lane >> 3) & 1) << 3), s + (lane >> 4)));
+          uint32_t a[2][4];
 #pragma unroll
           for (int u = 0; u < 2; u++) {
-            uint32_t a[4];
             if constexpr (kKeepQ) {
 #pragma unroll
-              for (int e = 0; e < 4; e++) a[e] = qf[s + u][e];
+              for (int e = 0; e < 4; e++) a[u][e] = qf[s + u][e];
             } else {
-              load_q(s + u, a);
+              load_q(s + u, a[u]);
             }
-            mma16816<false>(sc[0], a, e4m3_to_f16(kf[2 * u]), e4m3_to_f16(kf[2 * u] >> 16));
-            mma16816<false>(sc[1], a, e4m3_to_f16(kf[2 * u + 1]), e4m3_to_f16(kf[2 * u + 1] >> 16));
+          }
+#pragma unroll
+          for (int blk = 0; blk < kBlocks; blk++) {
+            // a 16-byte chunk is 16 values of a row, one step; a lane gets values 4 (lane & 3) to 4 (lane & 3) + 3
+            uint32_t kf[4];   // rows 0-7, 8-15 of step s; the same of step s + 1
+            ldsm4(kf, k_addr + chunk_at<S::kRowBytes>(w0 + blk * 16 + (lane & 7) + (((lane >> 3) & 1) << 3), s + (lane >> 4)));
+#pragma unroll
+            for (int u = 0; u < 2; u++)
+#pragma unroll
+              for (int n = 0; n < 2; n++) {
+                uint32_t b0, b1;
+                e4m3_to_f16(kf[2 * u + n], b0, b1);
+                if (kSets == 2 && u == 1) mma16816<false>(more[n], a[u], b0, b1);
+                else mma16816<false>(sc[blk][n], a[u], b0, b1);
+              }
           }
         }
       }
       // ---- base-2 scores, -inf for rows that are not there; running maximum
-      const uint32_t mask = masks[(i % S::kMasks) * 2 + (r0 >> 5)] >> (r0 & 31);
       float top[2] = {m_run[0], m_run[1]};
 #pragma unroll
-      for (int n = 0; n < 2; n++)
+      for (int blk = 0; blk < kBlocks; blk++) {
+        const int r0 = w0 + blk * 16;
+        const uint32_t mask = masks[stage * S::kMaskWords + (r0 >> 5)] >> ((r0 & 31) + (lane & 3) * 2);
 #pragma unroll
-        for (int e = 0; e < 4; e++) {
-          const int r = n * 8 + (lane & 3) * 2 + (e & 1);
-          sc[n][e] = (mask >> r) & 1u ? sc[n][e] * row_scale[e >> 1] : kNegInf;
-          top[e >> 1] = fmaxf(top[e >> 1], sc[n][e]);
-        }
+        for (int n = 0; n < 2; n++)
+#pragma unroll
+          for (int e = 0; e < 4; e++) {
+            const float x = kSets == 2 ? sc[blk][n][e] + more[n][e] : sc[blk][n][e];
+            sc[blk][n][e] = (mask >> (n * 8 + (e & 1))) & 1u ? x * row_scale[e >> 1] : kNegInf;
+            top[e >> 1] = fmaxf(top[e >> 1], sc[blk][n][e]);
+          }
+      }
       if (p.scores != nullptr) {
-        float* const to = p.scores + ((static_cast<int64_t>(range.first) + i) * p.chunk + wm * 16 + (lane >> 2)) * kKvTile + r0 + (lane & 3) * 2;
+        float* const to = p.scores + ((static_cast<int64_t>(range.first) + i) * p.chunk + wm * 16 + (lane >> 2)) * S::kTile + w0 + (lane & 3) * 2;
 #pragma unroll
         for (int half = 0; half < 2; half++) {
           if (wm * 16 + half * 8 + (lane >> 2) >= unit_heads) continue;
 #pragma unroll
-          for (int n = 0; n < 2; n++)
-            *reinterpret_cast<float2*>(to + half * 8 * kKvTile + n * 8) = make_float2(sc[n][2 * half], sc[n][2 * half + 1]);
+          for (int blk = 0; blk < kBlocks; blk++)
+#pragma unroll
+            for (int n = 0; n < 2; n++)
+              *reinterpret_cast<float2*>(to + half * 8 * S::kTile + blk * 16 + n * 8) =
+                  make_float2(sc[blk][n][2 * half], sc[blk][n][2 * half + 1]);
         }
       }
-      float base[2], fade[2];
+      float base[2] = {0.0f, 0.0f}, fade[2] = {1.0f, 1.0f};
 #pragma unroll
       for (int half = 0; half < 2; half++) {
-        if (half == 1 && !upper) {
-          base[1] = 0.0f;
-          fade[1] = 1.0f;
-          continue;
-        }
+        if (half == 1 && !upper) continue;
         top[half] = quad_max(top[half]);
         base[half] = top[half] == kNegInf ? 0.0f : top[half];
         fade[half] = exp2_fast(m_run[half] - base[half]);
@@ -459,53 +519,61 @@ __global__ void __launch_bounds__(kThreads, Shape<ST, DP, WM>::kMinCtas) attend_
         m_run[0] = top[0];
         if (upper) m_run[1] = top[1];
       }
-      float pr[2][4] = {};
+      // ---- probabilities and the weighted sum of values
+      uint32_t a[kBlocks][4];
 #pragma unroll
-      for (int half = 0; half < 2; half++) {
-        if (half == 1 && !upper) continue;
+      for (int blk = 0; blk < kBlocks; blk++) {
+        float pr[2][4] = {};
 #pragma unroll
-        for (int n = 0; n < 2; n++)
+        for (int half = 0; half < 2; half++) {
+          if (half == 1 && !upper) continue;
 #pragma unroll
-          for (int e = 0; e < 2; e++) {
-            pr[n][2 * half + e] = exp2_fast(sc[n][2 * half + e] - base[half]);
-            l_run[half] += pr[n][2 * half + e];
-          }
-      }
-      // ---- weighted sum of values
-      uint32_t a[4];
+          for (int n = 0; n < 2; n++)
 #pragma unroll
-      for (int n = 0; n < 2; n++) {
-        a[2 * n] = pack2<kBf16>(pr[n][0], pr[n][1]);
-        a[2 * n + 1] = pack2<kBf16>(pr[n][2], pr[n][3]);
+            for (int e = 0; e < 2; e++) {
+              pr[n][2 * half + e] = exp2_fast(sc[blk][n][2 * half + e] - base[half]);
+              l_run[half] += pr[n][2 * half + e];
+            }
+        }
+#pragma unroll
+        for (int n = 0; n < 2; n++) {
+          a[blk][2 * n] = pack2<kBf16>(pr[n][0], pr[n][1]);
+          a[blk][2 * n + 1] = pack2<kBf16>(pr[n][2], pr[n][3]);
+        }
       }
       if constexpr (!kE4m3) {
 #pragma unroll
-        for (int s = 0; s < kSteps; s++) {
-          uint32_t vf[4];   // rows 0-7, 8-15 of columns 0-7, then of columns 8-15
-          ldsm4_t(vf, v_addr + chunk_at<S::kRowBytes>(r0 + (lane & 15), s * 2 + (lane >> 4)));
-          mma16816<kBf16>(acc[s][0], a, vf[0], vf[1]);
-          mma16816<kBf16>(acc[s][1], a, vf[2], vf[3]);
-        }
+        for (int s = 0; s < kSteps; s++)
+#pragma unroll
+          for (int blk = 0; blk < kBlocks; blk++) {
+            uint32_t vf[4];   // rows 0-7, 8-15 of columns 0-7, then of columns 8-15
+            ldsm4_t(vf, v_addr + chunk_at<S::kRowBytes>(w0 + blk * 16 + (lane & 15), s * 2 + (lane >> 4)));
+            mma16816<kBf16>(acc[s][0], a[blk], vf[0], vf[1]);
+            mma16816<kBf16>(acc[s][1], a[blk], vf[2], vf[3]);
+          }
       } else {
 #pragma unroll
-        for (int s = 0; s < kSteps; s += 2) {
-          // transposed 16-bit units: a lane gets columns 2u, 2u + 1 (u = lane / 4) of two rows, byte by byte; the bytes
-          // are dealt out to the products of the even and of the odd columns
-          uint32_t vf[4];
-          ldsm4_t(vf, v_addr + chunk_at<S::kRowBytes>(r0 + (lane & 15), s + (lane >> 4)));
+        for (int s = 0; s < kSteps; s += 2)
 #pragma unroll
-          for (int u = 0; u < 2; u++) {
-            const uint32_t x = __byte_perm(vf[2 * u], 0, 0x3120), y = __byte_perm(vf[2 * u + 1], 0, 0x3120);
-            mma16816<false>(acc[s + u][0], a, e4m3_to_f16(x), e4m3_to_f16(y));
-            mma16816<false>(acc[s + u][1], a, e4m3_to_f16(x >> 16), e4m3_to_f16(y >> 16));
+          for (int blk = 0; blk < kBlocks; blk++) {
+            // transposed 16-bit units: a lane gets columns 2u, 2u + 1 (u = lane / 4) of two rows, byte by byte; the bytes
+            // are dealt out to the products of the even and of the odd columns
+            uint32_t vf[4];
+            ldsm4_t(vf, v_addr + chunk_at<S::kRowBytes>(w0 + blk * 16 + (lane & 15), s + (lane >> 4)));
+#pragma unroll
+            for (int u = 0; u < 2; u++) {
+              uint32_t even0, even1, odd0, odd1;
+              e4m3_to_f16(__byte_perm(vf[2 * u], 0, 0x3120), even0, odd0);
+              e4m3_to_f16(__byte_perm(vf[2 * u + 1], 0, 0x3120), even1, odd1);
+              mma16816<false>(acc[s + u][0], a[blk], even0, even1);
+              mma16816<false>(acc[s + u][1], a[blk], odd0, odd1);
+            }
           }
-        }
       }
     }
-    if (locates && tid < kKvTile) keep_located(ahead + 1, next);
 
     // ---- end of the unit, or of this CTA's part of it: join the warps that shared its rows
-    const bool to_end = use.j + 1 == use.tiles;
+    const bool to_end = at.j + 1 == at.tiles;
     if (to_end || i + 1 == n_tiles) {
       const bool whole = from_start && to_end;
       const float v_scale = kE4m3 && p.cache.value_scale != nullptr ? __ldg(p.cache.value_scale + head) : 1.0f;
@@ -514,10 +582,10 @@ __global__ void __launch_bounds__(kThreads, Shape<ST, DP, WM>::kMinCtas) attend_
         const float l = quad_sum(l_run[half]);
         if ((lane & 3) == 0) ml[warp * 16 + half * 8 + (lane >> 2)] = make_float2(m_run[half], l);
       }
-      __syncthreads();
-      float* const sums = reinterpret_cast<float*>(smem + (i % S::kStages) * 2 * S::kTileBytes);   // [4][8][DP]
-      const int64_t part = (static_cast<int64_t>(blockIdx.x) * 2 + part_slot(range.first, range.first + i - use.j)) * S::kUnitRows;
-      const int64_t unit_at = (static_cast<int64_t>(use.b) * units + use.unit) * S::kUnitRows;
+      compute_sync();                                       // every warp is done with this stage's tile
+      float* const sums = reinterpret_cast<float*>(smem + stage * 2 * S::kTileBytes);   // [warps][8][DP]
+      const int64_t part = (static_cast<int64_t>(blockIdx.x) * 2 + part_slot(range.first, range.first + i - at.j)) * S::kUnitRows;
+      const int64_t unit_at = (static_cast<int64_t>(at.b) * units + at.unit) * S::kUnitRows;
 #pragma unroll
       for (int half = 0; half < 2; half++) {
         if (half * 8 >= unit_heads) break;                  // (for every warp: rows of wm 0 come first)
@@ -545,8 +613,9 @@ __global__ void __launch_bounds__(kThreads, Shape<ST, DP, WM>::kMinCtas) attend_
             }
           }
         }
-        __syncthreads();
-        for (int rr = 0; rr < WM * 8; rr++) {
+        compute_sync();
+        // warp w puts out rows w, w + 4, ..
+        for (int rr = warp; rr < WM * 8; rr += kComputeWarps) {
           const int w = rr >> 3, row = rr & 7;
           const int hr = w * 16 + half * 8 + row;           // query head inside the unit
           if (hr >= unit_heads) continue;
@@ -561,27 +630,36 @@ __global__ void __launch_bounds__(kThreads, Shape<ST, DP, WM>::kMinCtas) attend_
           }
           const int q_head = head * p.group + unit_first + hr;
           const float inv = l == 0.0f ? 0.0f : v_scale / l;
-          for (int d = tid; d < width; d += kThreads) {
+#pragma unroll
+          for (int y = 0; y < DP / 32; y++) {
+            const int d = y * 32 + lane;
+            if (d >= width) break;
             float v = 0.0f;
 #pragma unroll
             for (int x = 0; x < S::kWT; x++) v += sums[((x * WM + w) * 8 + row) * DP + (d ^ ((row & 3) << 3))];
-            if (whole) store16(p.out + use.b * p.out_seq + q_head * p.out_head + d * 2, v * inv, p.q_bf16);
+            if (whole) store16(p.out + at.b * p.out_seq + q_head * p.out_head + d * 2, v * inv, p.q_bf16);
             else p.part_acc[(part + hr) * width + d] = v;
           }
-          if (tid == 0) {
+          if (lane == 0) {
             if (whole) {
               const float lse2 = l == 0.0f ? kNegInf : m + log2f(l);
               if (p.scores != nullptr) p.unit_lse[unit_at + hr] = lse2;
-              if (p.lse != nullptr) p.lse[static_cast<int64_t>(use.b) * p.q_heads + q_head] = lse2 * 0.69314718055994530942f;
+              if (p.lse != nullptr) p.lse[static_cast<int64_t>(at.b) * p.q_heads + q_head] = lse2 * 0.69314718055994530942f;
             } else {
               p.part_ml[part + hr] = make_float2(m, l);
             }
           }
         }
-        __syncthreads();
+        compute_sync();
       }
     }
-    use.advance(p.table, units);
+    __syncwarp();
+    if (lane == 0) mbar_arrive(empty + stage);
+    if (++stage == S::kStages) {
+      stage = 0;
+      phase ^= 1;
+    }
+    at.advance(p.table, units, S::kTile);
   }
 }
 

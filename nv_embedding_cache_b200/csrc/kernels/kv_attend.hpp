@@ -18,20 +18,21 @@ struct KvAttendParams {
   int32_t group;                     // query heads of one key head
   int32_t chunk;                     // query heads one unit takes (group split over `chunks` units)
   int32_t chunks;
+  int32_t tile_rows;                 // kv_tile_rows of this width and type
   int32_t rows_per_unit;             // padded rows of a unit in the scratch: 16, 32 or 64
   float scale_log2;                  // scale * log2(e)
   // scratch
   float* part_acc;                   // [ctas][2][rows_per_unit][width]
   float2* part_ml;                   // [ctas][2][rows_per_unit] (maximum, sum), base 2
   float* unit_lse;                   // [sequences * heads * chunks][rows_per_unit] base-2 lse of units one CTA did alone
-  float* scores;                     // [tiles][chunk][kKvTile] base-2 scores, nullptr without weights
+  float* scores;                     // [tiles][chunk][tile_rows] base-2 scores, nullptr without weights
   int32_t ctas;                      // grid of the split kernel
 };
 
 // Most CTAs the split kernel can use at once, for this variant on the current device.
 int kv_attend_resident(nve_data_type_t cache_dtype, int width, int rows_per_unit);
 void launch_kv_attend(const KvAttendParams& p, nve_data_type_t cache_dtype, cudaStream_t stream);
-void launch_kv_join(const KvAttendParams& p, int sms, cudaStream_t stream);
+void launch_kv_join(const KvAttendParams& p, cudaStream_t stream);
 
 // one per stored type, in a translation unit of its own
 template <typename ST>
@@ -47,7 +48,7 @@ struct TileCursor {
   int32_t length, tiles;             // of sequence b
 
   // Next tile; sequences without rows have none.
-  __device__ __forceinline__ void advance(const KvTable& t, int32_t units) {
+  __device__ __forceinline__ void advance(const KvTable& t, int32_t units, int32_t tile_rows) {
     if (++j < tiles) return;
     j = 0;
     if (++unit < units) return;
@@ -55,7 +56,7 @@ struct TileCursor {
     do {
       if (++b >= t.sequences) return;
       length = kv_length(t, b, nullptr);
-      tiles = tiles_of(length);
+      tiles = tiles_of(length, tile_rows);
     } while (tiles == 0);
   }
 };

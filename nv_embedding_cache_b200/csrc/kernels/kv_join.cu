@@ -2,10 +2,14 @@
 // into the weight every row drew.
 //
 // Join: out = sum_c 2^(m_c - M) acc_c / sum_c 2^(m_c - M) l_c over the CTAs c that had a part of the unit, M the
-// largest m_c; always in ascending c, so the result is the same on every run.  One block per (sequence, query head).
-// Weights: row j of key head h grows by sum_g 2^(x_gj - lse_g).  One warp per run of tiles, two rows a lane; the scores
-// were written by the first launch moments ago and mostly come from L2 (4 bytes per query head and row, against
-// 2 width values of the cache: 6 % of its bytes for eight heads on bf16 rows of 128).
+// largest m_c; added up in a fixed order, so the result is the same on every run.  One block per (sequence, query
+// head), its warps take the parts in turn.
+// Weights: row j of key head h grows by sum_g 2^(x_gj - lse_g).  One block per 1024 rows of a (sequence, key head), four
+// rows a thread.  The scores were written by the first launch moments ago and come from L2 as far as they fit
+// (4 bytes per query head and row, against 2 width values of the cache: 6 % of its bytes for four heads on bf16
+// rows of 128).
+// The launch overlaps the first one's end (programmatic dependent launch): what needs only the lengths is done before
+// the wait.
 #include <algorithm>
 
 #include "../common.hpp"
@@ -15,93 +19,102 @@ namespace nve_b200 {
 
 namespace {
 
-constexpr int kThreads = 128;
+constexpr int kThreads = 256;
+constexpr int kWarps = kThreads / 32;
+constexpr int kSlice = kThreads * 4;   // rows of a weight block
+constexpr int kMaxChunk = 64;          // query heads of a unit
 constexpr float kNegInf = -__builtin_huge_valf();
 
+// The CTAs that had a part of the unit that begins at tile `first_tile`, and where their parts are in the scratch: a
+// CTA's first part is slot 0, and only the first CTA of a unit can have it second.
 struct Parts {
-  int32_t first, last;               // CTAs that had a part of the unit
+  int32_t first, last;
+  int32_t first_slot;
+  __device__ __forceinline__ int64_t row(const KvAttendParams& p, int32_t c) const {
+    return (static_cast<int64_t>(c) * 2 + (c == first ? first_slot : 0)) * p.rows_per_unit;
+  }
 };
 __device__ __forceinline__ Parts parts_of(int64_t total, int32_t n, int32_t first_tile, int32_t tiles) {
-  return {cta_of_tile(total, n, first_tile), cta_of_tile(total, n, first_tile + tiles - 1)};
-}
-// Scratch row of the unit's part in CTA c: a CTA's first part is slot 0.
-__device__ __forceinline__ int64_t part_row(const KvAttendParams& p, int64_t total, int32_t n, int32_t c, int32_t first_tile) {
-  const int slot = part_slot(tile_range(total, n, c).first, first_tile);
-  return (static_cast<int64_t>(c) * 2 + slot) * p.rows_per_unit;
-}
-
-// Base-2 lse of query head `hr` of a unit.
-__device__ __forceinline__ float unit_lse2(const KvAttendParams& p, int64_t total, int32_t n, int32_t first_tile,
-                                           int32_t tiles, int64_t unit_row, int32_t hr) {
-  const Parts parts = parts_of(total, n, first_tile, tiles);
-  if (parts.first == parts.last) return p.unit_lse[unit_row + hr];
-  float m = kNegInf, l = 0.0f;
-  for (int32_t c = parts.first; c <= parts.last; c++) {
-    const float2 o = p.part_ml[part_row(p, total, n, c, first_tile) + hr];
-    const float top = fmaxf(m, o.x);
-    const float base = top == kNegInf ? 0.0f : top;
-    l = l * exp2f(m - base) + o.y * exp2f(o.x - base);
-    m = top;
-  }
-  return l == 0.0f ? kNegInf : m + log2f(l);
+  Parts r;
+  r.first = cta_of_tile(total, n, first_tile);
+  r.last = cta_of_tile(total, n, first_tile + tiles - 1);
+  r.first_slot = part_slot(tile_range(total, n, r.first).first, first_tile);
+  return r;
 }
 
-__global__ void __launch_bounds__(kThreads) join_kernel(const KvAttendParams p, int32_t join_blocks, int32_t weight_blocks) {
-  __shared__ int64_t s_sum[4];
+// (maximum, sum) of two runs together
+__device__ __forceinline__ float2 join_ml(float2 a, float2 b) {
+  const float m = fmaxf(a.x, b.x), base = m == kNegInf ? 0.0f : m;
+  return make_float2(m, a.y * exp2f(a.x - base) + b.y * exp2f(b.x - base));
+}
+
+// Waits for the end of the first launch.  Every block does, so that this grid never ends before that one.
+__device__ __forceinline__ void first_launch_done() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+
+__global__ void __launch_bounds__(kThreads) join_kernel(const KvAttendParams p, int32_t weight_blocks, int32_t slices) {
+  __shared__ int64_t s_sum[kWarps][2];
+  __shared__ float s_lse[kMaxChunk];
+  __shared__ float s_l[kWarps], s_acc[kWarps][256];
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int units = p.cache.heads * p.chunks;
-  const int me_x = static_cast<int>(blockIdx.x);
-  const int my_b = me_x < join_blocks ? me_x / p.q_heads : -1;
+  const int block = static_cast<int>(blockIdx.x);
+  const bool weights = block < weight_blocks;
+  const int list = weights ? block / slices : 0;            // (sequence, key head)
+  const int q_index = block - weight_blocks;                // (sequence, query head)
+  const int b = weights ? list / p.cache.heads : q_index / p.q_heads;
 
-  // tiles of all sequences, and of those before this block's
+  const int length = kv_length(p.table, b, nullptr);
+  const int tiles = tiles_of(length, p.tile_rows);
+  const int row0 = weights ? (block - list * slices) * kSlice : 0;
+  if (row0 >= length) {
+    first_launch_done();
+    return;
+  }
+  // tiles of all sequences, and of those before b
   int64_t all = 0, before = 0;
-  for (int b = tid; b < p.table.sequences; b += kThreads) {
-    const int nt = tiles_of(kv_length(p.table, b, nullptr));
+  for (int x = tid; x < p.table.sequences; x += kThreads) {
+    const int nt = tiles_of(kv_length(p.table, x, nullptr), p.tile_rows);
     all += nt;
-    if (b < my_b) before += nt;
+    if (x < b) before += nt;
   }
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) {
     all += __shfl_xor_sync(0xffffffffu, all, o);
     before += __shfl_xor_sync(0xffffffffu, before, o);
   }
-  if (lane == 0) s_sum[warp] = all;
+  if (lane == 0) {
+    s_sum[warp][0] = all;
+    s_sum[warp][1] = before;
+  }
   __syncthreads();
-  const int64_t sum_tiles = s_sum[0] + s_sum[1] + s_sum[2] + s_sum[3];
-  __syncthreads();
-  if (lane == 0) s_sum[warp] = before;
-  __syncthreads();
-  const int64_t before_tiles = s_sum[0] + s_sum[1] + s_sum[2] + s_sum[3];
-  const int64_t total = sum_tiles * units;
-  if (total == 0) return;
+  all = before = 0;
+#pragma unroll
+  for (int w = 0; w < kWarps; w++) {
+    all += s_sum[w][0];
+    before += s_sum[w][1];
+  }
+  const int64_t total = all * units;
   const int32_t n = static_cast<int32_t>(min(static_cast<int64_t>(p.ctas), total));
+  const int32_t seq_tile = static_cast<int32_t>(before * units);
 
-  if (my_b >= 0) {
+  if (!weights) {
     // ---- join of one query head
-    const int q_head = me_x - my_b * p.q_heads;
+    const int q_head = q_index - b * p.q_heads;
     const int head = q_head / p.group, in_group = q_head - head * p.group;
     const int chunk = in_group / p.chunk, hr = in_group - chunk * p.chunk;
-    const int tiles = tiles_of(kv_length(p.table, my_b, nullptr));
-    if (tiles == 0) return;
-    const int32_t first_tile = static_cast<int32_t>(before_tiles * units) + (head * p.chunks + chunk) * tiles;
-    const Parts parts = parts_of(total, n, first_tile, tiles);
+    const Parts parts = parts_of(total, n, seq_tile + (head * p.chunks + chunk) * tiles, tiles);
+    first_launch_done();
     if (parts.first == parts.last) return;                  // done by the CTA that had it alone
-    __shared__ float s_max[4], s_l[4], s_acc[4][256];
-    // warps take the parts in turn, each with its own maximum
     float m = kNegInf;
-    for (int32_t c = parts.first + tid; c <= parts.last; c += kThreads)
-      m = fmaxf(m, p.part_ml[part_row(p, total, n, c, first_tile) + hr].x);
+    for (int32_t c = parts.first + lane; c <= parts.last; c += 32) m = fmaxf(m, p.part_ml[parts.row(p, c) + hr].x);
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
-    if (lane == 0) s_max[warp] = m;
-    __syncthreads();
-    m = fmaxf(fmaxf(s_max[0], s_max[1]), fmaxf(s_max[2], s_max[3]));
     const float base = m == kNegInf ? 0.0f : m;
     float acc[8] = {};
     float l = 0.0f;
     const int width = p.cache.width;
-    for (int32_t c = parts.first + warp; c <= parts.last; c += 4) {
-      const int64_t row = part_row(p, total, n, c, first_tile) + hr;
+    for (int32_t c = parts.first + warp; c <= parts.last; c += kWarps) {
+      const int64_t row = parts.row(p, c) + hr;
       const float2 o = p.part_ml[row];
       const float f = exp2f(o.x - base);
       l += o.y * f;
@@ -115,103 +128,117 @@ __global__ void __launch_bounds__(kThreads) join_kernel(const KvAttendParams p, 
     for (int x = 0; x < 8; x++) s_acc[warp][x * 32 + lane] = acc[x];
     if (lane == 0) s_l[warp] = l;
     __syncthreads();
-    l = s_l[0] + s_l[1] + s_l[2] + s_l[3];
+    l = 0.0f;
+#pragma unroll
+    for (int w = 0; w < kWarps; w++) l += s_l[w];
     const float v_scale = p.cache.value_scale != nullptr ? __ldg(p.cache.value_scale + head) : 1.0f;
     const float inv = l == 0.0f ? 0.0f : v_scale / l;
-    for (int d = tid; d < width; d += kThreads) {
-      const float v = (s_acc[0][d] + s_acc[1][d] + s_acc[2][d] + s_acc[3][d]) * inv;
-      uint8_t* const to = p.out + my_b * p.out_seq + q_head * p.out_head + d * 2;
-      if (p.q_bf16) *reinterpret_cast<__nv_bfloat16*>(to) = __float2bfloat16_rn(v);
-      else *reinterpret_cast<__half*>(to) = __float2half_rn(v);
+    if (tid < width) {
+      float v = 0.0f;
+#pragma unroll
+      for (int w = 0; w < kWarps; w++) v += s_acc[w][tid];
+      uint8_t* const to = p.out + b * p.out_seq + q_head * p.out_head + tid * 2;
+      if (p.q_bf16) *reinterpret_cast<__nv_bfloat16*>(to) = __float2bfloat16_rn(v * inv);
+      else *reinterpret_cast<__half*>(to) = __float2half_rn(v * inv);
     }
     if (tid == 0 && p.lse != nullptr) {
-      p.lse[static_cast<int64_t>(my_b) * p.q_heads + q_head] = l == 0.0f ? kNegInf : (m + log2f(l)) * 0.69314718055994530942f;
+      p.lse[static_cast<int64_t>(b) * p.q_heads + q_head] = l == 0.0f ? kNegInf : (m + log2f(l)) * 0.69314718055994530942f;
     }
     return;
   }
 
-  // ---- weights: runs of (sequence, key head, tile), one per warp
-  const int64_t w_total = sum_tiles * p.cache.heads;
-  const int32_t warps = weight_blocks * 4, me = (me_x - join_blocks) * 4 + warp;
-  const TileRange range = tile_range(w_total, warps, me);
-  if (range.first == range.last) return;
-  TileCursor at{0, 0, 0, 0, 0};
-  int32_t seq_tile = 0;                                      // tiles of the sequences before at.b
-  {
-    int64_t seen = 0;
-    for (int b = 0; b < p.table.sequences; b += 32) {
-      const int mine = b + lane;
-      const int nt = mine < p.table.sequences ? tiles_of(kv_length(p.table, mine, nullptr)) : 0;
-      int64_t incl = nt;
+  // ---- weights of rows row0 to row0 + kSlice - 1
+  const int head = list - b * p.cache.heads;
+  const int row = row0 + tid * 4, there = min(4, length - row);   // there <= 0: none
+  const int tile = row / p.tile_rows, in_tile = row % p.tile_rows;
+  // where the weights are: four rows of one page in one piece, or row by row
+  const bool four = p.cache.page_size % 4 == 0 && reinterpret_cast<uint64_t>(p.cache.weights) % 16 == 0;
+  float* at[4] = {};
+  if (there > 0) {
 #pragma unroll
-      for (int o = 1; o < 32; o <<= 1) {
-        const int64_t x = __shfl_up_sync(0xffffffffu, incl, o);
-        if (lane >= o) incl += x;
-      }
-      const int64_t off = range.first - (seen + incl - nt) * p.cache.heads;
-      const bool found = off >= 0 && off < static_cast<int64_t>(nt) * p.cache.heads;
-      const uint32_t who = __ballot_sync(0xffffffffu, found);
-      if (who != 0) {
-        const int src = __ffs(who) - 1;
-        const int32_t o32 = __shfl_sync(0xffffffffu, static_cast<int32_t>(off), src);
-        at.b = b + src;
-        at.tiles = __shfl_sync(0xffffffffu, nt, src);
-        at.unit = o32 / at.tiles;
-        at.j = o32 % at.tiles;
-        seq_tile = static_cast<int32_t>(__shfl_sync(0xffffffffu, seen + incl - nt, src));
-        break;
-      }
-      seen += __shfl_sync(0xffffffffu, incl, 31);
+    for (int x = 0; x < 4; x++) {
+      if (x >= there || (x > 0 && four)) break;
+      int32_t slot;
+      const int32_t page = kv_locate(p.cache, p.table.pages, p.table.stride, b, row + x, &slot);
+      if (page >= 0) at[x] = p.cache.weights + kv_weight_index(p.cache, page, head, slot);
     }
   }
-  at.length = kv_length(p.table, at.b, nullptr);
-  float lse[2] = {};                                         // of query heads lane, lane + 32 of the chunk in use
-  int lse_b = -1, lse_unit = -1;
-  for (int32_t t = range.first; t < range.last; t++) {
-    const int row0 = at.j * kKvTile + lane * 2;
-    float w[2] = {0.0f, 0.0f};
-    for (int chunk = 0; chunk < p.chunks; chunk++) {
-      const int unit = at.unit * p.chunks + chunk;
-      const int32_t first_tile = seq_tile * units + unit * at.tiles;
-      const int heads = min(p.chunk, p.group - chunk * p.chunk);
-      if (lse_b != at.b || lse_unit != unit) {
-        const int64_t unit_row = (static_cast<int64_t>(at.b) * units + unit) * p.rows_per_unit;
+  first_launch_done();
+  float w[4] = {};
+  for (int chunk = 0; chunk < p.chunks; chunk++) {
+    const int unit = head * p.chunks + chunk;
+    const int32_t first_tile = seq_tile + unit * tiles;
+    const int heads = min(p.chunk, p.group - chunk * p.chunk);
+    const Parts parts = parts_of(total, n, first_tile, tiles);
+    if (chunk > 0) __syncthreads();
+    if (parts.first == parts.last) {
+      if (tid < heads) s_lse[tid] = p.unit_lse[(static_cast<int64_t>(b) * units + unit) * p.rows_per_unit + tid];
+    } else {
+      // eight lanes a head
+      for (int g0 = warp * 4; g0 < heads; g0 += kWarps * 4) {
+        const int g = g0 + (lane >> 3);
+        float2 ml = make_float2(kNegInf, 0.0f);
+        if (g < heads) {
+          for (int32_t c = parts.first + (lane & 7); c <= parts.last; c += 8) ml = join_ml(ml, p.part_ml[parts.row(p, c) + g]);
+        }
 #pragma unroll
-        for (int x = 0; x < 2; x++)
-          if (lane + 32 * x < heads) lse[x] = unit_lse2(p, total, n, first_tile, at.tiles, unit_row, lane + 32 * x);
-        lse_b = at.b;
-        lse_unit = unit;
+        for (int o = 4; o > 0; o >>= 1) {
+          const float2 other = make_float2(__shfl_xor_sync(0xffffffffu, ml.x, o), __shfl_xor_sync(0xffffffffu, ml.y, o));
+          ml = join_ml(ml, other);
+        }
+        if ((lane & 7) == 0 && g < heads) s_lse[g] = ml.y == 0.0f ? kNegInf : ml.x + log2f(ml.y);
       }
-      const float* const s = p.scores + (static_cast<int64_t>(first_tile) + at.j) * p.chunk * kKvTile + lane * 2;
+    }
+    __syncthreads();
+    if (there > 0) {
+      const float* const s = p.scores + (static_cast<int64_t>(first_tile) + tile) * p.chunk * p.tile_rows + in_tile;
+#pragma unroll 8
       for (int g = 0; g < heads; g++) {
-        const float e = __shfl_sync(0xffffffffu, g < 32 ? lse[0] : lse[1], g & 31);
-        if (row0 < at.length && e != kNegInf) {
-          const float2 x = *reinterpret_cast<const float2*>(s + g * kKvTile);
+        const float4 x = *reinterpret_cast<const float4*>(s + g * p.tile_rows);
+        const float e = s_lse[g];
+        if (e != kNegInf) {
           w[0] += exp2f(x.x - e);
           w[1] += exp2f(x.y - e);
+          w[2] += exp2f(x.z - e);
+          w[3] += exp2f(x.w - e);
         }
       }
     }
-#pragma unroll
-    for (int x = 0; x < 2; x++) {
-      if (row0 + x < at.length) {
-        int32_t slot;
-        const int32_t page = kv_locate(p.cache, p.table.pages, p.table.stride, at.b, row0 + x, &slot);
-        if (page >= 0) p.cache.weights[kv_weight_index(p.cache, page, at.unit, slot)] += w[x];
-      }
+  }
+  if (there == 4 && four) {
+    if (at[0] != nullptr) {
+      float4 v = *reinterpret_cast<float4*>(at[0]);
+      v.x += w[0];
+      v.y += w[1];
+      v.z += w[2];
+      v.w += w[3];
+      *reinterpret_cast<float4*>(at[0]) = v;
     }
-    if (at.j + 1 == at.tiles && at.unit + 1 == p.cache.heads) seq_tile += at.tiles;
-    at.advance(p.table, p.cache.heads);
+  } else {
+#pragma unroll
+    for (int x = 0; x < 4; x++) {
+      if (x >= there) break;
+      float* const to = four ? (at[0] == nullptr ? nullptr : at[0] + x) : at[x];
+      if (to != nullptr) *to += w[x];
+    }
   }
 }
 
 }  // namespace
 
-void launch_kv_join(const KvAttendParams& p, int sms, cudaStream_t stream) {
-  const int32_t join_blocks = p.table.sequences * p.q_heads;
-  const int32_t weight_blocks = p.scores != nullptr ? sms * 8 : 0;
-  join_kernel<<<join_blocks + weight_blocks, kThreads, 0, stream>>>(p, join_blocks, weight_blocks);
-  NVE_B200_CUDA(cudaGetLastError());
+void launch_kv_join(const KvAttendParams& p, cudaStream_t stream) {
+  const int32_t slices = p.scores != nullptr ? static_cast<int32_t>(ceil_div(p.table.capacity, kSlice)) : 0;
+  const int32_t weight_blocks = p.table.sequences * p.cache.heads * slices;
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3(static_cast<unsigned>(weight_blocks + p.table.sequences * p.q_heads));
+  cfg.blockDim = dim3(kThreads);
+  cfg.stream = stream;
+  cudaLaunchAttribute attr{};
+  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr.val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = &attr;
+  cfg.numAttrs = 1;
+  NVE_B200_CUDA(cudaLaunchKernelEx(&cfg, join_kernel, p, weight_blocks, std::max(slices, 1)));
 }
 
 int kv_attend_resident(nve_data_type_t cache_dtype, int width, int rows_per_unit) {

@@ -32,13 +32,19 @@ NVE_KV_FN uint32_t fast_div(uint32_t n, const FastDiv& f) {
 }
 
 // ---- tiles of the attention -----------------------------------------------------------------------
-// Tiles (64 rows of one unit = a key head and a chunk of its query heads) are numbered sequence by sequence, inside
+// Tiles (kv_tile_rows rows of one unit = a key head and a chunk of its query heads) are numbered sequence by sequence, inside
 // a sequence unit by unit, inside a unit along the length.  CTA c of n takes the run [c total / n, (c + 1) total / n):
 // every CTA gets the same number of tiles, give or take one, whatever the lengths are.  n <= total, so no run is empty.
-constexpr int kKvTile = 64;
+// Rows of a tile: 16 KB of keys and 16 KB of values for rows of 128 and 256 bytes (the width is padded to 64, 128 or
+// 256 values); 128 rows at most, so that short sequences still make several tiles.
+constexpr int kKvMaxTile = 128;
+NVE_KV_FN constexpr int kv_padded_width(int width) { return width <= 64 ? 64 : (width <= 128 ? 128 : 256); }
+NVE_KV_FN constexpr int kv_tile_rows(int width, int value_bytes) {
+  return kv_padded_width(width) * value_bytes <= 128 ? kKvMaxTile : 64;
+}
 
-NVE_KV_FN int32_t tiles_of(int32_t length) {
-  return static_cast<int32_t>((static_cast<int64_t>(length) + kKvTile - 1) / kKvTile);
+NVE_KV_FN int32_t tiles_of(int32_t length, int32_t tile_rows) {   // a power of two
+  return static_cast<int32_t>((static_cast<uint32_t>(length) + tile_rows - 1) / static_cast<uint32_t>(tile_rows));
 }
 
 struct TileRange {

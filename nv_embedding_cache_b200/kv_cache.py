@@ -221,7 +221,8 @@ class PagedKVCache:
         if bits:
             self.status.zero_()
             what = [text for bit, text in ((capi.KV_BAD_PAGE, "a page id outside the pool"),
-                                           (capi.KV_BAD_LENGTH, "a length outside the page table or max_length"))
+                                           (capi.KV_BAD_LENGTH, "a length outside the page table or max_length"),
+                                           (capi.KV_TIMED_OUT, "a wait that ran into its limit"))
                     if bits & bit]
             raise RuntimeError("paged cache: " + " and ".join(what))
 

@@ -5,7 +5,8 @@ using namespace nve_b200;
 
 extern "C" {
 uint32_t kp_div(uint32_t n, uint32_t d) { return fast_div(n, make_fast_div(d)); }
-int32_t kp_tiles(int32_t length) { return tiles_of(length); }
+int32_t kp_tiles(int32_t length, int32_t rows) { return tiles_of(length, rows); }
+int32_t kp_tile_rows(int32_t width, int32_t bytes) { return kv_tile_rows(width, bytes); }
 void kp_range(int64_t total, int32_t n, int32_t c, int32_t* out) {
   const TileRange r = tile_range(total, n, c);
   out[0] = r.first;

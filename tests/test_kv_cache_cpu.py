@@ -76,7 +76,10 @@ def test_unfinished_units_of_a_run_have_slots_of_their_own(plan):
 
 
 def test_tiles_of_lengths(plan):
-    assert [plan.kp_tiles(x) for x in (0, 1, 63, 64, 65, 128, 129, (1 << 31) - 1)] == [0, 1, 1, 1, 2, 2, 3, 1 << 25]
+    assert [plan.kp_tiles(x, 64) for x in (0, 1, 63, 64, 65, 128, 129, (1 << 31) - 1)] == [0, 1, 1, 1, 2, 2, 3, 1 << 25]
+    assert [plan.kp_tiles(x, 128) for x in (0, 1, 128, 129, (1 << 31) - 1)] == [0, 1, 1, 2, 1 << 24]
+    assert [plan.kp_tile_rows(w, b) for w, b in ((8, 2), (64, 2), (72, 2), (128, 2), (256, 2), (128, 1), (136, 1))] == \
+        [128, 128, 64, 64, 64, 128, 64]
 
 
 # ---- refusals ------------------------------------------------------------------------------------
