@@ -272,7 +272,7 @@ void attend(const nve_b200_kv_cache_t* cache, const nve_b200_kv_attend_t* a, voi
   p.q_bf16 = a->dtype == NVE_DTYPE_BFLOAT16;
   p.scale_log2 = a->scale * 1.44269504088896340736f;
   launch_kv_attend(p, cache->dtype, stream);
-  launch_kv_join(p, stream);
+  launch_kv_join(p, sm_count(), stream);
 }
 
 void evict(const nve_b200_kv_cache_t* cache, const nve_b200_kv_evict_t* a, cudaStream_t stream) {

@@ -43,6 +43,9 @@ constexpr float kNegInf = -__builtin_huge_valf();
 __device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, bool take) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(take ? 16 : 0) : "memory");
 }
+__device__ __forceinline__ void cp_async16_full(uint32_t dst, const void* src) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+}
 // The barrier gets this thread's arrival when its copies so far are done.
 __device__ __forceinline__ void cp_async_arrive(uint64_t* bar) {
   asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(smem_addr(bar)) : "memory");
@@ -225,7 +228,8 @@ __global__ void __launch_bounds__(kThreads, Shape<ST, DP, WM>::kMinCtas) attend_
   __syncthreads();
   TileCursor at;
   at.b = s_start[0];
-  at.unit = s_start[1];
+  at.head = s_start[1] / p.chunks;
+  at.chunk = s_start[1] - at.head * p.chunks;
   at.j = s_start[2];
   at.length = kv_length(p.table, at.b, nullptr);
   at.tiles = tiles_of(at.length, S::kTile);
@@ -242,23 +246,29 @@ __global__ void __launch_bounds__(kThreads, Shape<ST, DP, WM>::kMinCtas) attend_
     const int lw = warp - kComputeWarps;
     const int row_chunks = width * static_cast<int>(sizeof(ST)) / 16, q_chunks = width / 8;
     longlong2* const own = offs + lw * kOwnRows;
-    // byte offsets of this lane's rows of the tile `at`; negative: no such row
+    // addresses of this lane's rows (keys, values) of the tile `at`; 0: no such row
     auto locate = [&](longlong2 (&o)[kEach]) {
-      const int32_t head = at.unit / p.chunks;
 #pragma unroll
       for (int x = 0; x < kEach; x++) {
         const int32_t row = at.j * S::kTile + lw * kOwnRows + x * 32 + lane;
-        o[x] = make_longlong2(-1, -1);
+        o[x] = make_longlong2(0, 0);
         if (row < at.length) {
           int32_t slot;
           const int32_t page = kv_locate(p.cache, p.table.pages, p.table.stride, at.b, row, &slot);
           if (page >= 0) {
-            o[x].x = page * p.cache.k_page + slot * p.cache.k_slot + head * p.cache.k_head;
-            o[x].y = page * p.cache.v_page + slot * p.cache.v_slot + head * p.cache.v_head;
+            o[x].x = reinterpret_cast<int64_t>(p.cache.keys) + page * p.cache.k_page + slot * p.cache.k_slot + at.head * p.cache.k_head;
+            o[x].y = reinterpret_cast<int64_t>(p.cache.values) + page * p.cache.v_page + slot * p.cache.v_slot + at.head * p.cache.v_head;
           }
         }
       }
     };
+    // A step of the warp copies 32 chunks, kRowsStep whole rows.  The permutation of the chunks repeats every 8 rows, so
+    // a lane's place in the stage is one of kPeriod bases and a constant.
+    static_assert(S::kChunks <= 32, "a row is at most one step");
+    constexpr int kRowsStep = 32 / S::kChunks;
+    constexpr int kPeriod = 8 / kRowsStep;
+    constexpr int kCopies = kOwnRows / kRowsStep;
+    const int r_lane = lane / S::kChunks, c_lane = lane % S::kChunks;
     longlong2 next[kEach];
     locate(next);
     int q_at = 0;                                           // buffer of the unit's queries
@@ -269,37 +279,53 @@ __global__ void __launch_bounds__(kThreads, Shape<ST, DP, WM>::kMinCtas) attend_
         break;
       }
       __syncwarp();
+      bool all_there = row_chunks == S::kChunks;
 #pragma unroll
       for (int x = 0; x < kEach; x++) {
         own[x * 32 + lane] = next[x];
-        const uint32_t mask = __ballot_sync(0xffffffffu, next[x].x >= 0);
+        const uint32_t mask = __ballot_sync(0xffffffffu, next[x].x != 0);
         if (lane == 0) masks[stage * S::kMaskWords + lw * kEach + x] = mask;
+        all_there = all_there && mask == 0xffffffffu;
       }
       __syncwarp();
       if (lane == 0) mbar_arrive(full + stage);
       const bool first = i == 0 || at.j == 0;
       const TileCursor now = at;
-      at.advance(p.table, units, S::kTile);
+      at.advance(p.table, p.cache.heads, p.chunks, S::kTile);
       if (i + 1 < n_tiles) locate(next);                    // its page ids arrive while this tile's copies are issued
-      const uint32_t k_addr = smem_addr(smem) + stage * 2 * S::kTileBytes, v_addr = k_addr + S::kTileBytes;
-#pragma unroll 8
-      for (int x = 0; x < kOwnRows * S::kChunks / 32; x++) {
-        const int id = x * 32 + lane;
-        const int r = id / S::kChunks, c = id % S::kChunks;
-        const longlong2 o = own[r];
-        // chunks behind the row's width and rows that are not there become zeros: a NaN left in a page never meets
-        // the products
-        const bool ok = o.x >= 0 && c < row_chunks;
-        const uint32_t to = chunk_at<S::kRowBytes>(lw * kOwnRows + r, c);
-        cp_async16(k_addr + to, p.cache.keys + (ok ? o.x + c * 16 : 0), ok);
-        cp_async16(v_addr + to, p.cache.values + (ok ? o.y + c * 16 : 0), ok);
+      const uint32_t k_addr = smem_addr(smem) + stage * 2 * S::kTileBytes + lw * kOwnRows * S::kRowBytes;
+      if (all_there) {
+#pragma unroll
+        for (int y = 0; y < kPeriod; y++) {
+          const uint32_t to = k_addr + chunk_at<S::kRowBytes>(y * kRowsStep + r_lane, c_lane);
+          const longlong2* const from = own + y * kRowsStep + r_lane;
+#pragma unroll
+          for (int x = 0; x < kCopies / kPeriod; x++) {
+            const longlong2 o = from[x * 8];
+            const uint32_t dst = to + x * 8 * S::kRowBytes;
+            cp_async16_full(dst, reinterpret_cast<const uint8_t*>(o.x) + c_lane * 16);
+            cp_async16_full(dst + S::kTileBytes, reinterpret_cast<const uint8_t*>(o.y) + c_lane * 16);
+          }
+        }
+      } else {
+#pragma unroll 2
+        for (int x = 0; x < kCopies; x++) {
+          const int r = x * kRowsStep + r_lane;
+          const longlong2 o = own[r];
+          // chunks behind the row's width and rows that are not there become zeros: a NaN left in a page never meets
+          // the products
+          const bool ok = o.x != 0 && c_lane < row_chunks;
+          const uint32_t dst = k_addr + chunk_at<S::kRowBytes>(r, c_lane);
+          cp_async16(dst, ok ? reinterpret_cast<const uint8_t*>(o.x) + c_lane * 16 : p.cache.keys, ok);
+          cp_async16(dst + S::kTileBytes, ok ? reinterpret_cast<const uint8_t*>(o.y) + c_lane * 16 : p.cache.values, ok);
+        }
       }
       if (first) {                                          // the unit's queries
         if (i > 0) q_at = q_at + 1 == S::kStages ? 0 : q_at + 1;
         const uint32_t q_addr = smem_addr(qbuf) + q_at * S::kQBytes;
-        const int head = now.unit / p.chunks, q_first = (now.unit % p.chunks) * p.chunk;
+        const int q_first = now.chunk * p.chunk;
         const int n = min(p.chunk, p.group - q_first);
-        const uint8_t* const src = p.q + now.b * p.q_seq + (head * p.group + q_first) * p.q_head;
+        const uint8_t* const src = p.q + now.b * p.q_seq + (now.head * p.group + q_first) * p.q_head;
         for (int id = lw * 32 + lane; id < S::kUnitRows * (DP / 8); id += kLoadWarps * 32) {
           const int r = id / (DP / 8), c = id % (DP / 8);
           const bool ok = r < n && c < q_chunks;
@@ -332,8 +358,8 @@ __global__ void __launch_bounds__(kThreads, Shape<ST, DP, WM>::kMinCtas) attend_
       kv_flag(p.cache.status, NVE_B200_KV_TIMED_OUT);
       return;
     }
-    const int head = at.unit / p.chunks;
-    const int unit_first = (at.unit % p.chunks) * p.chunk;  // first query head of the unit inside its group
+    const int head = at.head;
+    const int unit_first = at.chunk * p.chunk;              // first query head of the unit inside its group
     const int unit_heads = min(p.chunk, p.group - unit_first);
     const bool lower = wm * 16 < unit_heads, upper = wm * 16 + 8 < unit_heads;   // rows 0-7, 8-15 hold heads
     auto load_q = [&](int step, uint32_t (&a)[4]) {
@@ -473,19 +499,38 @@ __global__ void __launch_bounds__(kThreads, Shape<ST, DP, WM>::kMinCtas) attend_
       }
       // ---- base-2 scores, -inf for rows that are not there; running maximum
       float top[2] = {m_run[0], m_run[1]};
+      uint32_t there[kBlocks];
+      bool all_there = true;
 #pragma unroll
       for (int blk = 0; blk < kBlocks; blk++) {
         const int r0 = w0 + blk * 16;
-        const uint32_t mask = masks[stage * S::kMaskWords + (r0 >> 5)] >> ((r0 & 31) + (lane & 3) * 2);
+        there[blk] = (masks[stage * S::kMaskWords + (r0 >> 5)] >> (r0 & 31)) & 0xffffu;
+        all_there = all_there && there[blk] == 0xffffu;
+      }
+#pragma unroll
+      for (int blk = 0; blk < kBlocks; blk++)
 #pragma unroll
         for (int n = 0; n < 2; n++)
 #pragma unroll
           for (int e = 0; e < 4; e++) {
             const float x = kSets == 2 ? sc[blk][n][e] + more[n][e] : sc[blk][n][e];
-            sc[blk][n][e] = (mask >> (n * 8 + (e & 1))) & 1u ? x * row_scale[e >> 1] : kNegInf;
-            top[e >> 1] = fmaxf(top[e >> 1], sc[blk][n][e]);
+            sc[blk][n][e] = x * row_scale[e >> 1];
           }
+      if (!all_there) {                                     // uniform in the warp
+#pragma unroll
+        for (int blk = 0; blk < kBlocks; blk++)
+#pragma unroll
+          for (int n = 0; n < 2; n++)
+#pragma unroll
+            for (int e = 0; e < 4; e++)
+              if (!((there[blk] >> (n * 8 + (lane & 3) * 2 + (e & 1))) & 1u)) sc[blk][n][e] = kNegInf;
       }
+#pragma unroll
+      for (int blk = 0; blk < kBlocks; blk++)
+#pragma unroll
+        for (int n = 0; n < 2; n++)
+#pragma unroll
+          for (int e = 0; e < 4; e++) top[e >> 1] = fmaxf(top[e >> 1], sc[blk][n][e]);
       if (p.scores != nullptr) {
         float* const to = p.scores + ((static_cast<int64_t>(range.first) + i) * p.chunk + wm * 16 + (lane >> 2)) * S::kTile + w0 + (lane & 3) * 2;
 #pragma unroll
@@ -585,7 +630,7 @@ __global__ void __launch_bounds__(kThreads, Shape<ST, DP, WM>::kMinCtas) attend_
       compute_sync();                                       // every warp is done with this stage's tile
       float* const sums = reinterpret_cast<float*>(smem + stage * 2 * S::kTileBytes);   // [warps][8][DP]
       const int64_t part = (static_cast<int64_t>(blockIdx.x) * 2 + part_slot(range.first, range.first + i - at.j)) * S::kUnitRows;
-      const int64_t unit_at = (static_cast<int64_t>(at.b) * units + at.unit) * S::kUnitRows;
+      const int64_t unit_at = (static_cast<int64_t>(at.b) * units + head * p.chunks + at.chunk) * S::kUnitRows;
 #pragma unroll
       for (int half = 0; half < 2; half++) {
         if (half * 8 >= unit_heads) break;                  // (for every warp: rows of wm 0 come first)
@@ -659,7 +704,7 @@ __global__ void __launch_bounds__(kThreads, Shape<ST, DP, WM>::kMinCtas) attend_
       stage = 0;
       phase ^= 1;
     }
-    at.advance(p.table, units, S::kTile);
+    at.advance(p.table, p.cache.heads, p.chunks, S::kTile);
   }
 }
 

@@ -32,7 +32,7 @@ struct KvAttendParams {
 // Most CTAs the split kernel can use at once, for this variant on the current device.
 int kv_attend_resident(nve_data_type_t cache_dtype, int width, int rows_per_unit);
 void launch_kv_attend(const KvAttendParams& p, nve_data_type_t cache_dtype, cudaStream_t stream);
-void launch_kv_join(const KvAttendParams& p, cudaStream_t stream);
+void launch_kv_join(const KvAttendParams& p, int sms, cudaStream_t stream);
 
 // one per stored type, in a translation unit of its own
 template <typename ST>
@@ -44,15 +44,17 @@ struct KvAttendVariant {
 #ifdef __CUDACC__
 // The walk over tiles in the order of kv_plan.hpp.
 struct TileCursor {
-  int32_t b, unit, j;                // sequence, unit inside the sequence, tile inside the unit
+  int32_t b, head, chunk, j;         // sequence, key head, chunk of its query heads, tile inside the unit
   int32_t length, tiles;             // of sequence b
 
   // Next tile; sequences without rows have none.
-  __device__ __forceinline__ void advance(const KvTable& t, int32_t units, int32_t tile_rows) {
+  __device__ __forceinline__ void advance(const KvTable& t, int32_t heads, int32_t chunks, int32_t tile_rows) {
     if (++j < tiles) return;
     j = 0;
-    if (++unit < units) return;
-    unit = 0;
+    if (++chunk < chunks) return;
+    chunk = 0;
+    if (++head < heads) return;
+    head = 0;
     do {
       if (++b >= t.sequences) return;
       length = kv_length(t, b, nullptr);

@@ -2,12 +2,14 @@
 // into the weight every row drew.
 //
 // Join: out = sum_c 2^(m_c - M) acc_c / sum_c 2^(m_c - M) l_c over the CTAs c that had a part of the unit, M the
-// largest m_c; added up in a fixed order, so the result is the same on every run.  One block per (sequence, query
-// head), its warps take the parts in turn.
-// Weights: row j of key head h grows by sum_g 2^(x_gj - lse_g).  One block per 1024 rows of a (sequence, key head), four
-// rows a thread.  The scores were written by the first launch moments ago and come from L2 as far as they fit
-// (4 bytes per query head and row, against 2 width values of the cache: 6 % of its bytes for four heads on bf16
-// rows of 128).
+// largest m_c; added up in a fixed order, so the result is the same on every run.  A block takes 1, 2, 4 or 8 query
+// heads of a unit, 8, 4, 2 or 1 warps each: one head where units are few and their parts many, eight where it is the
+// other way round.
+// Weights: row j of key head h grows by sum_g 2^(x_gj - lse_g).  A block takes a slice of the rows of a (sequence, key
+// head), four rows a thread and step.  The scores were written by the first launch moments ago and come from L2 as
+// far as they fit (4 bytes per query head and row, against 2 width values of the cache: 6 % of its bytes for eight
+// heads on bf16 rows of 128).  What a block does before its first score (tiles before its sequence, the lse of its
+// heads) is a chain of waits, so slices are as long as filling the GPU allows.
 // The launch overlaps the first one's end (programmatic dependent launch): what needs only the lengths is done before
 // the wait.
 #include <algorithm>
@@ -21,7 +23,7 @@ namespace {
 
 constexpr int kThreads = 256;
 constexpr int kWarps = kThreads / 32;
-constexpr int kSlice = kThreads * 4;   // rows of a weight block
+constexpr int kStep = kThreads * 4;    // rows a weight block takes at once
 constexpr int kMaxChunk = 64;          // query heads of a unit
 constexpr float kNegInf = -__builtin_huge_valf();
 
@@ -51,21 +53,28 @@ __device__ __forceinline__ float2 join_ml(float2 a, float2 b) {
 // Waits for the end of the first launch.  Every block does, so that this grid never ends before that one.
 __device__ __forceinline__ void first_launch_done() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 
-__global__ void __launch_bounds__(kThreads) join_kernel(const KvAttendParams p, int32_t weight_blocks, int32_t slices) {
+struct JoinPlan {
+  int32_t weight_blocks;             // the first blocks: slices of rows
+  int32_t slices;                    // of a (sequence, key head)
+  int32_t slice_rows;                // a multiple of kStep
+  int32_t heads;                     // query heads of a join block: 1, 2, 4 or 8
+  int32_t per_unit;                  // join blocks of a unit
+};
+
+__global__ void __launch_bounds__(kThreads) join_kernel(const KvAttendParams p, const JoinPlan plan) {
   __shared__ int64_t s_sum[kWarps][2];
   __shared__ float s_lse[kMaxChunk];
   __shared__ float s_l[kWarps], s_acc[kWarps][256];
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int units = p.cache.heads * p.chunks;
   const int block = static_cast<int>(blockIdx.x);
-  const bool weights = block < weight_blocks;
-  const int list = weights ? block / slices : 0;            // (sequence, key head)
-  const int q_index = block - weight_blocks;                // (sequence, query head)
-  const int b = weights ? list / p.cache.heads : q_index / p.q_heads;
+  const bool weights = block < plan.weight_blocks;
+  const int list = weights ? block / plan.slices : (block - plan.weight_blocks) / plan.per_unit;   // (sequence, key head), or (sequence, unit)
+  const int b = list / (weights ? p.cache.heads : units);
 
   const int length = kv_length(p.table, b, nullptr);
   const int tiles = tiles_of(length, p.tile_rows);
-  const int row0 = weights ? (block - list * slices) * kSlice : 0;
+  const int row0 = weights ? (block - list * plan.slices) * plan.slice_rows : 0;
   if (row0 >= length) {
     first_launch_done();
     return;
@@ -98,73 +107,82 @@ __global__ void __launch_bounds__(kThreads) join_kernel(const KvAttendParams p, 
   const int32_t seq_tile = static_cast<int32_t>(before * units);
 
   if (!weights) {
-    // ---- join of one query head
-    const int q_head = q_index - b * p.q_heads;
-    const int head = q_head / p.group, in_group = q_head - head * p.group;
-    const int chunk = in_group / p.chunk, hr = in_group - chunk * p.chunk;
-    const Parts parts = parts_of(total, n, seq_tile + (head * p.chunks + chunk) * tiles, tiles);
+    // ---- join of some query heads of a unit
+    const int unit = list - b * units;
+    const Parts parts = parts_of(total, n, seq_tile + unit * tiles, tiles);
     first_launch_done();
     if (parts.first == parts.last) return;                  // done by the CTA that had it alone
-    float m = kNegInf;
-    for (int32_t c = parts.first + lane; c <= parts.last; c += 32) m = fmaxf(m, p.part_ml[parts.row(p, c) + hr].x);
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
-    const float base = m == kNegInf ? 0.0f : m;
-    float acc[8] = {};
-    float l = 0.0f;
+    const int head = unit / p.chunks, chunk = unit - head * p.chunks;
+    const int shares = kWarps / plan.heads;                 // warps of a query head
+    const int share = warp % shares;
+    const int hr = (block - plan.weight_blocks - list * plan.per_unit) * plan.heads + warp / shares;
+    const bool mine = hr < min(p.chunk, p.group - chunk * p.chunk);
     const int width = p.cache.width;
-    for (int32_t c = parts.first + warp; c <= parts.last; c += kWarps) {
-      const int64_t row = parts.row(p, c) + hr;
-      const float2 o = p.part_ml[row];
-      const float f = exp2f(o.x - base);
-      l += o.y * f;
+    float m = kNegInf, l = 0.0f;
+    if (mine) {
+      for (int32_t c = parts.first + lane; c <= parts.last; c += 32) m = fmaxf(m, p.part_ml[parts.row(p, c) + hr].x);
 #pragma unroll
-      for (int x = 0; x < 8; x++) {
-        const int d = x * 32 + lane;
-        if (d < width) acc[x] += p.part_acc[row * width + d] * f;
+      for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+      const float base = m == kNegInf ? 0.0f : m;
+      float acc[8] = {};
+      for (int32_t c = parts.first + share; c <= parts.last; c += shares) {
+        const int64_t row = parts.row(p, c) + hr;
+        const float2 o = p.part_ml[row];
+        const float f = exp2f(o.x - base);
+        l += o.y * f;
+#pragma unroll
+        for (int x = 0; x < 8; x++) {
+          const int d = x * 32 + lane;
+          if (d < width) acc[x] += p.part_acc[row * width + d] * f;
+        }
       }
+#pragma unroll
+      for (int x = 0; x < 8; x++) s_acc[warp][x * 32 + lane] = acc[x];
+      if (lane == 0) s_l[warp] = l;
     }
-#pragma unroll
-    for (int x = 0; x < 8; x++) s_acc[warp][x * 32 + lane] = acc[x];
-    if (lane == 0) s_l[warp] = l;
     __syncthreads();
+    if (!mine) return;
     l = 0.0f;
-#pragma unroll
-    for (int w = 0; w < kWarps; w++) l += s_l[w];
+    for (int w = 0; w < shares; w++) l += s_l[warp - share + w];
     const float v_scale = p.cache.value_scale != nullptr ? __ldg(p.cache.value_scale + head) : 1.0f;
     const float inv = l == 0.0f ? 0.0f : v_scale / l;
-    if (tid < width) {
+    const int q_head = head * p.group + chunk * p.chunk + hr;
+    for (int d = share * 32 + lane; d < width; d += shares * 32) {
       float v = 0.0f;
-#pragma unroll
-      for (int w = 0; w < kWarps; w++) v += s_acc[w][tid];
-      uint8_t* const to = p.out + b * p.out_seq + q_head * p.out_head + tid * 2;
+      for (int w = 0; w < shares; w++) v += s_acc[warp - share + w][d];
+      uint8_t* const to = p.out + b * p.out_seq + q_head * p.out_head + d * 2;
       if (p.q_bf16) *reinterpret_cast<__nv_bfloat16*>(to) = __float2bfloat16_rn(v * inv);
       else *reinterpret_cast<__half*>(to) = __float2half_rn(v * inv);
     }
-    if (tid == 0 && p.lse != nullptr) {
+    if (share == 0 && lane == 0 && p.lse != nullptr) {
       p.lse[static_cast<int64_t>(b) * p.q_heads + q_head] = l == 0.0f ? kNegInf : (m + log2f(l)) * 0.69314718055994530942f;
     }
     return;
   }
 
-  // ---- weights of rows row0 to row0 + kSlice - 1
+  // ---- weights of a slice of rows
   const int head = list - b * p.cache.heads;
-  const int row = row0 + tid * 4, there = min(4, length - row);   // there <= 0: none
-  const int tile = row / p.tile_rows, in_tile = row % p.tile_rows;
-  // where the weights are: four rows of one page in one piece, or row by row
+  const int slice_end = min(row0 + plan.slice_rows, length);
+  // four rows of one page are one piece of memory where pages hold fours
   const bool four = p.cache.page_size % 4 == 0 && reinterpret_cast<uint64_t>(p.cache.weights) % 16 == 0;
-  float* at[4] = {};
-  if (there > 0) {
+  float* at[4];
+  // where the weights of the four rows from `row` on are; nullptr: not there
+  auto find = [&](int row) {
 #pragma unroll
     for (int x = 0; x < 4; x++) {
-      if (x >= there || (x > 0 && four)) break;
+      at[x] = nullptr;
+      if (row + x >= length) continue;
+      if (x > 0 && four) {
+        at[x] = at[0] == nullptr ? nullptr : at[0] + x;
+        continue;
+      }
       int32_t slot;
       const int32_t page = kv_locate(p.cache, p.table.pages, p.table.stride, b, row + x, &slot);
       if (page >= 0) at[x] = p.cache.weights + kv_weight_index(p.cache, page, head, slot);
     }
-  }
+  };
+  find(row0 + tid * 4);
   first_launch_done();
-  float w[4] = {};
   for (int chunk = 0; chunk < p.chunks; chunk++) {
     const int unit = head * p.chunks + chunk;
     const int32_t first_tile = seq_tile + unit * tiles;
@@ -190,8 +208,14 @@ __global__ void __launch_bounds__(kThreads) join_kernel(const KvAttendParams p, 
       }
     }
     __syncthreads();
-    if (there > 0) {
+    for (int row = row0 + tid * 4; row < slice_end; row += kStep) {
+      if (chunk > 0 || row >= row0 + kStep) find(row);
+      float4 old = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+      const bool piece = four && at[3] != nullptr;
+      if (piece) old = *reinterpret_cast<const float4*>(at[0]);
+      const int tile = row / p.tile_rows, in_tile = row % p.tile_rows;
       const float* const s = p.scores + (static_cast<int64_t>(first_tile) + tile) * p.chunk * p.tile_rows + in_tile;
+      float w[4] = {};
 #pragma unroll 8
       for (int g = 0; g < heads; g++) {
         const float4 x = *reinterpret_cast<const float4*>(s + g * p.tile_rows);
@@ -203,34 +227,34 @@ __global__ void __launch_bounds__(kThreads) join_kernel(const KvAttendParams p, 
           w[3] += exp2f(x.w - e);
         }
       }
-    }
-  }
-  if (there == 4 && four) {
-    if (at[0] != nullptr) {
-      float4 v = *reinterpret_cast<float4*>(at[0]);
-      v.x += w[0];
-      v.y += w[1];
-      v.z += w[2];
-      v.w += w[3];
-      *reinterpret_cast<float4*>(at[0]) = v;
-    }
-  } else {
+      if (piece) {
+        *reinterpret_cast<float4*>(at[0]) = make_float4(old.x + w[0], old.y + w[1], old.z + w[2], old.w + w[3]);
+      } else {
 #pragma unroll
-    for (int x = 0; x < 4; x++) {
-      if (x >= there) break;
-      float* const to = four ? (at[0] == nullptr ? nullptr : at[0] + x) : at[x];
-      if (to != nullptr) *to += w[x];
+        for (int x = 0; x < 4; x++)
+          if (at[x] != nullptr) *at[x] += w[x];
+      }
     }
   }
 }
 
 }  // namespace
 
-void launch_kv_join(const KvAttendParams& p, cudaStream_t stream) {
-  const int32_t slices = p.scores != nullptr ? static_cast<int32_t>(ceil_div(p.table.capacity, kSlice)) : 0;
-  const int32_t weight_blocks = p.table.sequences * p.cache.heads * slices;
+void launch_kv_join(const KvAttendParams& p, int sms, cudaStream_t stream) {
+  const int64_t lists = static_cast<int64_t>(p.table.sequences) * p.cache.heads;
+  const int64_t unit_count = lists * p.chunks;
+  JoinPlan plan{};
+  // slices: four blocks per SM (as many as run at once) if the rows are enough for that
+  const int64_t most = std::max<int64_t>(1, ceil_div(p.table.capacity, kStep));
+  const int64_t wanted = std::min<int64_t>(most, std::max<int64_t>(1, int64_t{4} * sms / lists));
+  plan.slice_rows = static_cast<int32_t>(ceil_div(most, wanted) * kStep);
+  plan.slices = static_cast<int32_t>(std::max<int64_t>(1, ceil_div(p.table.capacity, plan.slice_rows)));
+  plan.weight_blocks = p.scores != nullptr ? static_cast<int32_t>(lists * plan.slices) : 0;
+  plan.heads = 1;
+  while (plan.heads < kWarps && plan.heads < p.chunk && unit_count * ceil_div(p.chunk, plan.heads) > sms) plan.heads *= 2;
+  plan.per_unit = static_cast<int32_t>(ceil_div(p.chunk, plan.heads));
   cudaLaunchConfig_t cfg{};
-  cfg.gridDim = dim3(static_cast<unsigned>(weight_blocks + p.table.sequences * p.q_heads));
+  cfg.gridDim = dim3(static_cast<unsigned>(plan.weight_blocks + unit_count * plan.per_unit));
   cfg.blockDim = dim3(kThreads);
   cfg.stream = stream;
   cudaLaunchAttribute attr{};
@@ -238,7 +262,7 @@ void launch_kv_join(const KvAttendParams& p, cudaStream_t stream) {
   attr.val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = &attr;
   cfg.numAttrs = 1;
-  NVE_B200_CUDA(cudaLaunchKernelEx(&cfg, join_kernel, p, weight_blocks, std::max(slices, 1)));
+  NVE_B200_CUDA(cudaLaunchKernelEx(&cfg, join_kernel, p, plan));
 }
 
 int kv_attend_resident(nve_data_type_t cache_dtype, int width, int rows_per_unit) {
