@@ -227,7 +227,7 @@ void attend(const nve_b200_kv_cache_t* cache, const nve_b200_kv_attend_t* a, voi
   p.group = a->num_q_heads / cache->num_heads;
   p.chunks = static_cast<int32_t>(ceil_div(p.group, 64));
   p.chunk = static_cast<int32_t>(ceil_div(p.group, p.chunks));
-  p.rows_per_unit = p.chunk <= 16 ? 16 : (p.chunk <= 32 ? 32 : 64);
+  p.rows_per_unit = p.chunk <= 8 ? 8 : (p.chunk <= 16 ? 16 : (p.chunk <= 32 ? 32 : 64));
   const int64_t units = static_cast<int64_t>(cache->num_heads) * p.chunks;
   p.tile_rows = kv_tile_rows(cache->head_width, static_cast<int>(value_bytes(cache->dtype)));
   const int64_t tiles = a->num_sequences * units * ceil_div(p.table.capacity, p.tile_rows);

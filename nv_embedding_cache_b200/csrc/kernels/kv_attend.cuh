@@ -13,11 +13,13 @@
 //    the page table and fill the ring with cp.async (16 bytes each: a page may end anywhere in a tile, rows have
 //    any strides), four warps compute; full and empty barriers per stage, no barrier over all warps.  The ring
 //    runs on across units, the queries of a unit travel with its first tile.
-//  * mma.sync m16n8k16, not tcgen05: a tile has as few as one query row, a 128-row tcgen05 tile would be 8 to
-//    128 times padding and its accumulator would have to leave TMEM for the running maximum every 64 rows.  Here
-//    the scores stay in the registers that the second product takes them from.
-// With up to 16 query heads each of the four warps takes a quarter of the tile's rows and has its own running maximum,
-// and the four are joined when the unit ends; with more, warps take 16 heads each and share the rows.
+//  * mma.sync m16n8k16, not tcgen05, with the cache as the left operand: keys (16 rows x 16 values) times queries
+//    (16 values x 8 heads), values transposed (16 values x 16 rows) times probabilities (16 rows x 8 heads).  A unit has as
+//    few as one query head; eight columns are the least there is, and the scores stay in the registers that the second
+//    product takes them from (transposed by movmatrix).  In a tcgen05 product they would go through TMEM and shared
+//    memory every tile, for a rate that the loads cannot feed.
+// With up to 16 query heads each computing warp takes its share of the tile's rows and has its own running maximum, and the
+// warps are joined when the unit ends; with more, warps take 16 heads each and share the rows.
 //
 // Probabilities are rounded to the type of the values (f16 for E4M3 rows: exact for them, see below) before the
 // second product: relative 2^-9 (bf16) or 2^-12 of each, below the rounding of the output; the sum is taken before that.
@@ -75,6 +77,12 @@ __device__ __forceinline__ void mma16816(float (&c)[4], const uint32_t (&a)[4], 
                  : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
   }
 }
+// 8x8 matrix of 16-bit values, a row per four lanes, transposed
+__device__ __forceinline__ uint32_t transposed(uint32_t x) {
+  uint32_t y;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+  return y;
+}
 template <bool BF16>
 __device__ __forceinline__ uint32_t pack2(float lo, float hi) {
   if constexpr (BF16) {
@@ -100,17 +108,21 @@ __device__ __forceinline__ void store16(uint8_t* p, float x, bool bf16) {
   if (bf16) *reinterpret_cast<__nv_bfloat16*>(p) = __float2bfloat16_rn(x);
   else *reinterpret_cast<__half*>(p) = __float2half_rn(x);
 }
-__device__ __forceinline__ float quad_max(float x) {
-  x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 1));
-  return fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 2));
+// over the lanes that hold the same columns (rows lane / 4)
+__device__ __forceinline__ float column_max(float x) {
+#pragma unroll
+  for (int o = 4; o < 32; o <<= 1) x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, o));
+  return x;
 }
-__device__ __forceinline__ float quad_sum(float x) {
-  x += __shfl_xor_sync(0xffffffffu, x, 1);
-  return x + __shfl_xor_sync(0xffffffffu, x, 2);
+__device__ __forceinline__ float column_sum(float x) {
+#pragma unroll
+  for (int o = 4; o < 32; o <<= 1) x += __shfl_xor_sync(0xffffffffu, x, o);
+  return x;
 }
 
-// ST: stored type.  DP: width rounded up to 64, 128 or 256.  WM: warps along the query heads.
-template <typename ST, int DP, int WM>
+// ST: stored type.  DP: width rounded up to 64, 128 or 256.  WM: warps along the query heads.  NT: columns of 8 heads of a
+// warp.
+template <typename ST, int DP, int WM, int NT>
 struct Shape {
   static constexpr bool kE4m3 = sizeof(ST) == 1;
   static constexpr int kRowBytes = DP * sizeof(ST);
@@ -119,7 +131,7 @@ struct Shape {
   static constexpr int kTileBytes = kTile * kRowBytes;    // keys or values of a tile
   static constexpr int kWT = kComputeWarps / WM;          // warps along the rows
   static constexpr int kWarpRows = kTile / kWT;           // rows of a tile one warp takes
-  static constexpr int kUnitRows = 16 * WM;               // query rows
+  static constexpr int kUnitRows = 8 * NT * WM;           // query rows
   static constexpr int kQBytes = kUnitRows * DP * 2;
   // A stage holds a tile and the queries of the unit that may begin with it.  Two CTAs per SM of three or more stages
   // where they fit, else one: 130 KB and more in flight per SM; the memory's latency times its rate asks for 45 KB.
@@ -129,7 +141,7 @@ struct Shape {
                                                : (222000 / kStageBytes < 5 ? 222000 / kStageBytes : 5);
   static constexpr int kMaskWords = kTile / 32;
   static constexpr int kOffsBytes = kTile * 16;
-  static constexpr int kSmem = kStages * kStageBytes + kOffsBytes + kComputeWarps * 16 * 8 + kStages * kMaskWords * 4 +
+  static constexpr int kSmem = kStages * kStageBytes + kOffsBytes + kComputeWarps * 8 * NT * 8 + kStages * kMaskWords * 4 +
                                kUnitRows * 4 + kStages * 16 + 16;
   static_assert(kStages >= 2, "stages");
 };
@@ -142,9 +154,10 @@ __device__ __forceinline__ uint32_t chunk_at(int r, int c) {
   else return r * ROW_BYTES + ((c ^ ((r >> 1) & 3)) << 4);       // 64-byte rows: two per 128 bytes
 }
 
-template <typename ST, int DP, int WM>
-__global__ void __launch_bounds__(kThreads, Shape<ST, DP, WM>::kMinCtas) attend_kernel(const KvAttendParams p) {
-  using S = Shape<ST, DP, WM>;
+template <typename ST, int DP, int WM, int NT>
+__global__ void __launch_bounds__(kThreads, Shape<ST, DP, WM, NT>::kMinCtas) attend_kernel(const KvAttendParams p) {
+  using S = Shape<ST, DP, WM, NT>;
+  constexpr int kHeads = 8 * NT;                           // query heads of a warp
   constexpr bool kE4m3 = S::kE4m3;
   constexpr bool kBf16 = std::is_same<ST, __nv_bfloat16>::value;
   constexpr int kSteps = DP / 16;                          // k steps of the first product, column blocks of the second
@@ -155,8 +168,8 @@ __global__ void __launch_bounds__(kThreads, Shape<ST, DP, WM>::kMinCtas) attend_
   longlong2* const offs = reinterpret_cast<longlong2*>(qbuf + S::kStages * S::kQBytes);             // [kTile]
   uint64_t* const full = reinterpret_cast<uint64_t*>(reinterpret_cast<uint8_t*>(offs) + S::kOffsBytes);   // [kStages]
   uint64_t* const empty = full + S::kStages;                                                        // [kStages]
-  float2* const ml = reinterpret_cast<float2*>(empty + S::kStages);                                 // [warps][16]
-  uint32_t* const masks = reinterpret_cast<uint32_t*>(ml + kComputeWarps * 16);                     // [kStages][kMaskWords]
+  float2* const ml = reinterpret_cast<float2*>(empty + S::kStages);                                 // [warps][kHeads]
+  uint32_t* const masks = reinterpret_cast<uint32_t*>(ml + kComputeWarps * kHeads);                 // [kStages][kMaskWords]
   float* const q_up = reinterpret_cast<float*>(masks + S::kStages * S::kMaskWords);                 // [kUnitRows]
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int width = p.cache.width;
@@ -344,60 +357,71 @@ __global__ void __launch_bounds__(kThreads, Shape<ST, DP, WM>::kMinCtas) attend_
   }
 
   // ================================ computing warps ================================
-  const int wm = warp % WM, wt = warp / WM;                 // heads 16 wm.., rows kWarpRows wt.. of the tile
-  float acc[kSteps][2][4];
-  float m_run[2], l_run[2];
-  uint32_t qf[kKeepQ ? kSteps : 1][4];
-  float row_scale[2];
+  const int wm = warp % WM, wt = warp / WM;                 // heads kHeads wm.., rows kWarpRows wt.. of the tile
+  const int row = lane >> 2, col = (lane & 3) * 2;          // of a product's 16 x 8 results: rows row, row + 8, columns col, col + 1
+  float acc[kSteps][NT][4];                                 // values x heads
+  float m_run[NT][2], l_run[NT][2];                         // of heads col, col + 1; the sum of this lane's rows
+  uint32_t qf[kKeepQ ? kSteps : 1][NT][2];
+  float scale[NT][2];
   bool from_start = false;                                  // this CTA has the current unit from its first tile
   int q_use = 0;
 
 #pragma unroll 1
   for (int i = 0; i < n_tiles; i++) {
-    if (!mbar_wait_bounded(full + stage, phase)) {          // all four warps wait for the same event: all give up
+    if (!mbar_wait_bounded(full + stage, phase)) {          // all warps wait for the same event: all give up
       kv_flag(p.cache.status, NVE_B200_KV_TIMED_OUT);
       return;
     }
     const int head = at.head;
     const int unit_first = at.chunk * p.chunk;              // first query head of the unit inside its group
     const int unit_heads = min(p.chunk, p.group - unit_first);
-    const bool lower = wm * 16 < unit_heads, upper = wm * 16 + 8 < unit_heads;   // rows 0-7, 8-15 hold heads
-    auto load_q = [&](int step, uint32_t (&a)[4]) {
+    // queries of one step (16 values): the two registers of head `row` of each column block
+    auto load_q = [&](int step, uint32_t (&b)[NT][2]) {
       const uint32_t base = smem_addr(qbuf) + q_use * S::kQBytes;
-      if constexpr (!kE4m3) {
-        // rows 0-7, 8-15 of columns 0-7 of the step, then of columns 8-15
-        ldsm4(a, base + chunk_at<DP * 2>(wm * 16 + (lane & 15), step * 2 + (lane >> 4)));
-      } else {
-        // a lane gets four consecutive values of an E4M3 row; the columns of q are dealt out alike
-        const int c = step * 2 + ((lane & 3) >> 1), in = (lane & 1) * 8;
+      if constexpr (kE4m3) {
+        // a lane gets four consecutive values of an E4M3 row; the values of q are dealt out alike
 #pragma unroll
-        for (int half = 0; half < 2; half++) {
-          const uint32_t addr = base + chunk_at<DP * 2>(wm * 16 + (lane >> 2) + half * 8, c) + in;
-          asm volatile("ld.shared.v2.u32 {%0, %1}, [%2];" : "=r"(a[half]), "=r"(a[half + 2]) : "r"(addr) : "memory");
+        for (int n = 0; n < NT; n++) {
+          const uint32_t addr = base + chunk_at<DP * 2>(wm * kHeads + n * 8 + row, step * 2 + ((lane & 3) >> 1)) + (lane & 1) * 8;
+          asm volatile("ld.shared.v2.u32 {%0, %1}, [%2];" : "=r"(b[n][0]), "=r"(b[n][1]) : "r"(addr) : "memory");
         }
+      } else {
+#pragma unroll
+        for (int n = 0; n < NT; n++)
+#pragma unroll
+          for (int x = 0; x < 2; x++) {
+            const uint32_t addr = base + chunk_at<DP * 2>(wm * kHeads + n * 8 + row, step * 2 + x) + col * 2;
+            asm volatile("ld.shared.u32 %0, [%1];" : "=r"(b[n][x]) : "r"(addr) : "memory");
+          }
       }
     };
     if (i == 0 || at.j == 0) {
       if (i > 0) q_use = q_use + 1 == S::kStages ? 0 : q_use + 1;
       from_start = at.j == 0;
 #pragma unroll
-      for (int s = 0; s < kSteps; s++)
+      for (int n = 0; n < NT; n++) {
 #pragma unroll
-        for (int e = 0; e < 4; e++) acc[s][0][e] = acc[s][1][e] = 0.0f;
-      m_run[0] = m_run[1] = kNegInf;
-      l_run[0] = l_run[1] = 0.0f;
-      row_scale[0] = row_scale[1] = p.scale_log2;
+        for (int s = 0; s < kSteps; s++)
+#pragma unroll
+          for (int e = 0; e < 4; e++) acc[s][n][e] = 0.0f;
+#pragma unroll
+        for (int e = 0; e < 2; e++) {
+          m_run[n][e] = kNegInf;
+          l_run[n][e] = 0.0f;
+          scale[n][e] = p.scale_log2;
+        }
+      }
       if constexpr (kE4m3) {
         // Queries meet E4M3 rows as f16.  bf16 ones are brought into its range row by row: divided by the power of
         // two of the row's largest value, which the scores get back; exact but for values 2^-24 below that.
         if (p.q_bf16) {
           for (int r = warp; r < S::kUnitRows; r += kComputeWarps) {
-            uint32_t* const row = reinterpret_cast<uint32_t*>(qbuf + q_use * S::kQBytes) + r * (DP / 2);
+            uint32_t* const words = reinterpret_cast<uint32_t*>(qbuf + q_use * S::kQBytes) + r * (DP / 2);
             float2 v[DP / 64];
             uint32_t top = 0;
 #pragma unroll
             for (int x = 0; x < DP / 64; x++) {
-              const uint32_t w = row[x * 32 + lane];
+              const uint32_t w = words[x * 32 + lane];
               v[x] = make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u));
               const uint32_t ea = (__float_as_uint(v[x].x) >> 23) & 255u, eb = (__float_as_uint(v[x].y) >> 23) & 255u;
               top = max(top, max(ea == 255u ? 0u : ea, eb == 255u ? 0u : eb));
@@ -407,17 +431,21 @@ __global__ void __launch_bounds__(kThreads, Shape<ST, DP, WM>::kMinCtas) attend_
             top = min(top, 253u);
             const float down = __uint_as_float((254u - top) << 23);
 #pragma unroll
-            for (int x = 0; x < DP / 64; x++) row[x * 32 + lane] = pack2<false>(v[x].x * down, v[x].y * down);
+            for (int x = 0; x < DP / 64; x++) words[x * 32 + lane] = pack2<false>(v[x].x * down, v[x].y * down);
             if (lane == 0) q_up[r] = __uint_as_float(top << 23);
           }
           compute_sync();
-          row_scale[0] *= q_up[wm * 16 + (lane >> 2)];
-          row_scale[1] *= q_up[wm * 16 + (lane >> 2) + 8];
+#pragma unroll
+          for (int n = 0; n < NT; n++)
+#pragma unroll
+            for (int e = 0; e < 2; e++) scale[n][e] *= q_up[wm * kHeads + n * 8 + col + e];
         }
         if (p.cache.key_scale != nullptr) {
           const float s = __ldg(p.cache.key_scale + head);
-          row_scale[0] *= s;
-          row_scale[1] *= s;
+#pragma unroll
+          for (int n = 0; n < NT; n++)
+#pragma unroll
+            for (int e = 0; e < 2; e++) scale[n][e] *= s;
         }
       }
       if constexpr (kKeepQ) {
@@ -430,54 +458,50 @@ __global__ void __launch_bounds__(kThreads, Shape<ST, DP, WM>::kMinCtas) attend_
     const int left = at.length - at.j * S::kTile;           // rows of the tile that exist
     const int w0 = wt * S::kWarpRows;
 
-    if (w0 < left && lower) {                               // uniform in the warp
-      // ---- scores of 16 heads x kWarpRows rows; one block alone is added up in two halves, so that the products
+    if (w0 < left && wm * kHeads < unit_heads) {            // uniform in the warp
+      // ---- scores of kWarpRows rows x kHeads heads; one block alone is added up in two halves, so that the products
       // do not wait for one another
-      constexpr int kSets = kBlocks == 1 ? 2 : 1;
-      float sc[kBlocks][2][4];
-      float more[2][4];
+      constexpr int kSets = kBlocks * NT == 1 ? 2 : 1;
+      float sc[kBlocks][NT][4];
+      float more[4] = {};
 #pragma unroll
-      for (int n = 0; n < 2; n++)
+      for (int blk = 0; blk < kBlocks; blk++)
 #pragma unroll
-        for (int e = 0; e < 4; e++) {
-          more[n][e] = 0.0f;
+        for (int n = 0; n < NT; n++)
 #pragma unroll
-          for (int blk = 0; blk < kBlocks; blk++) sc[blk][n][e] = 0.0f;
-        }
+          for (int e = 0; e < 4; e++) sc[blk][n][e] = 0.0f;
       if constexpr (!kE4m3) {
 #pragma unroll
         for (int s = 0; s < kSteps; s++) {
-          uint32_t a[4];
+          uint32_t b[NT][2];
           if constexpr (kKeepQ) {
 #pragma unroll
-            for (int e = 0; e < 4; e++) a[e] = qf[s][e];
+            for (int n = 0; n < NT; n++) b[n][0] = qf[s][n][0], b[n][1] = qf[s][n][1];
           } else {
-            load_q(s, a);
+            load_q(s, b);
           }
 #pragma unroll
           for (int blk = 0; blk < kBlocks; blk++) {
-            uint32_t kf[4];   // rows 0-7: columns 0-7, 8-15 of the step; rows 8-15: the same
-            ldsm4(kf, k_addr + chunk_at<S::kRowBytes>(w0 + blk * 16 + (lane & 7) + ((lane >> 4) << 3), s * 2 + ((lane >> 3) & 1)));
-            if (kSets == 2 && (s & 1)) {
-              mma16816<kBf16>(more[0], a, kf[0], kf[1]);
-              mma16816<kBf16>(more[1], a, kf[2], kf[3]);
-            } else {
-              mma16816<kBf16>(sc[blk][0], a, kf[0], kf[1]);
-              mma16816<kBf16>(sc[blk][1], a, kf[2], kf[3]);
+            uint32_t a[4];    // rows 0-7, 8-15 of values 0-7 of the step, then of values 8-15
+            ldsm4(a, k_addr + chunk_at<S::kRowBytes>(w0 + blk * 16 + (lane & 15), s * 2 + (lane >> 4)));
+#pragma unroll
+            for (int n = 0; n < NT; n++) {
+              if (kSets == 2 && (s & 1)) mma16816<kBf16>(more, a, b[n][0], b[n][1]);
+              else mma16816<kBf16>(sc[blk][n], a, b[n][0], b[n][1]);
             }
           }
         }
       } else {
 #pragma unroll
         for (int s = 0; s < kSteps; s += 2) {
-          uint32_t a[2][4];
+          uint32_t b[2][NT][2];
 #pragma unroll
           for (int u = 0; u < 2; u++) {
             if constexpr (kKeepQ) {
 #pragma unroll
-              for (int e = 0; e < 4; e++) a[u][e] = qf[s + u][e];
+              for (int n = 0; n < NT; n++) b[u][n][0] = qf[s + u][n][0], b[u][n][1] = qf[s + u][n][1];
             } else {
-              load_q(s + u, a[u]);
+              load_q(s + u, b[u]);
             }
           }
 #pragma unroll
@@ -486,19 +510,20 @@ __global__ void __launch_bounds__(kThreads, Shape<ST, DP, WM>::kMinCtas) attend_
             uint32_t kf[4];   // rows 0-7, 8-15 of step s; the same of step s + 1
             ldsm4(kf, k_addr + chunk_at<S::kRowBytes>(w0 + blk * 16 + (lane & 7) + (((lane >> 3) & 1) << 3), s + (lane >> 4)));
 #pragma unroll
-            for (int u = 0; u < 2; u++)
+            for (int u = 0; u < 2; u++) {
+              uint32_t a[4];
+              e4m3_to_f16(kf[2 * u], a[0], a[2]);
+              e4m3_to_f16(kf[2 * u + 1], a[1], a[3]);
 #pragma unroll
-              for (int n = 0; n < 2; n++) {
-                uint32_t b0, b1;
-                e4m3_to_f16(kf[2 * u + n], b0, b1);
-                if (kSets == 2 && u == 1) mma16816<false>(more[n], a[u], b0, b1);
-                else mma16816<false>(sc[blk][n], a[u], b0, b1);
+              for (int n = 0; n < NT; n++) {
+                if (kSets == 2 && u == 1) mma16816<false>(more, a, b[u][n][0], b[u][n][1]);
+                else mma16816<false>(sc[blk][n], a, b[u][n][0], b[u][n][1]);
               }
+            }
           }
         }
       }
       // ---- base-2 scores, -inf for rows that are not there; running maximum
-      float top[2] = {m_run[0], m_run[1]};
       uint32_t there[kBlocks];
       bool all_there = true;
 #pragma unroll
@@ -510,108 +535,99 @@ __global__ void __launch_bounds__(kThreads, Shape<ST, DP, WM>::kMinCtas) attend_
 #pragma unroll
       for (int blk = 0; blk < kBlocks; blk++)
 #pragma unroll
-        for (int n = 0; n < 2; n++)
+        for (int n = 0; n < NT; n++)
 #pragma unroll
-          for (int e = 0; e < 4; e++) {
-            const float x = kSets == 2 ? sc[blk][n][e] + more[n][e] : sc[blk][n][e];
-            sc[blk][n][e] = x * row_scale[e >> 1];
-          }
+          for (int e = 0; e < 4; e++) sc[blk][n][e] = (kSets == 2 ? sc[blk][n][e] + more[e] : sc[blk][n][e]) * scale[n][e & 1];
       if (!all_there) {                                     // uniform in the warp
 #pragma unroll
         for (int blk = 0; blk < kBlocks; blk++)
 #pragma unroll
-          for (int n = 0; n < 2; n++)
+          for (int n = 0; n < NT; n++)
 #pragma unroll
             for (int e = 0; e < 4; e++)
-              if (!((there[blk] >> (n * 8 + (lane & 3) * 2 + (e & 1))) & 1u)) sc[blk][n][e] = kNegInf;
+              if (!((there[blk] >> (row + (e >> 1) * 8)) & 1u)) sc[blk][n][e] = kNegInf;
       }
+      if (p.scores != nullptr) {
+        float* const to = p.scores + ((static_cast<int64_t>(range.first) + i) * p.chunk + wm * kHeads + col) * S::kTile + w0 + row;
+#pragma unroll
+        for (int n = 0; n < NT; n++)
+#pragma unroll
+          for (int e = 0; e < 2; e++) {
+            if (wm * kHeads + n * 8 + col + e >= unit_heads) continue;
+#pragma unroll
+            for (int blk = 0; blk < kBlocks; blk++) {
+              to[(n * 8 + e) * S::kTile + blk * 16] = sc[blk][n][e];
+              to[(n * 8 + e) * S::kTile + blk * 16 + 8] = sc[blk][n][e + 2];
+            }
+          }
+      }
+      float base[NT][2], fade[NT][2];
+      bool moved = false;
+#pragma unroll
+      for (int n = 0; n < NT; n++)
+#pragma unroll
+        for (int e = 0; e < 2; e++) {
+          float top = m_run[n][e];
+#pragma unroll
+          for (int blk = 0; blk < kBlocks; blk++) top = fmaxf(top, fmaxf(sc[blk][n][e], sc[blk][n][e + 2]));
+          top = column_max(top);
+          base[n][e] = top == kNegInf ? 0.0f : top;
+          fade[n][e] = exp2_fast(m_run[n][e] - base[n][e]);
+          moved = moved || top != m_run[n][e];
+          m_run[n][e] = top;
+        }
+      if (__any_sync(0xffffffffu, moved)) {
+#pragma unroll
+        for (int n = 0; n < NT; n++) {
+#pragma unroll
+          for (int s = 0; s < kSteps; s++)
+#pragma unroll
+            for (int e = 0; e < 4; e++) acc[s][n][e] *= fade[n][e & 1];
+          l_run[n][0] *= fade[n][0];
+          l_run[n][1] *= fade[n][1];
+        }
+      }
+      // ---- probabilities and the weighted sum of values
+      uint32_t b[kBlocks][NT][2];
 #pragma unroll
       for (int blk = 0; blk < kBlocks; blk++)
 #pragma unroll
-        for (int n = 0; n < 2; n++)
+        for (int n = 0; n < NT; n++) {
+          float pr[4];
 #pragma unroll
-          for (int e = 0; e < 4; e++) top[e >> 1] = fmaxf(top[e >> 1], sc[blk][n][e]);
-      if (p.scores != nullptr) {
-        float* const to = p.scores + ((static_cast<int64_t>(range.first) + i) * p.chunk + wm * 16 + (lane >> 2)) * S::kTile + w0 + (lane & 3) * 2;
-#pragma unroll
-        for (int half = 0; half < 2; half++) {
-          if (wm * 16 + half * 8 + (lane >> 2) >= unit_heads) continue;
-#pragma unroll
-          for (int blk = 0; blk < kBlocks; blk++)
-#pragma unroll
-            for (int n = 0; n < 2; n++)
-              *reinterpret_cast<float2*>(to + half * 8 * S::kTile + blk * 16 + n * 8) =
-                  make_float2(sc[blk][n][2 * half], sc[blk][n][2 * half + 1]);
+          for (int e = 0; e < 4; e++) {
+            pr[e] = exp2_fast(sc[blk][n][e] - base[n][e & 1]);
+            l_run[n][e & 1] += pr[e];
+          }
+          b[blk][n][0] = transposed(pack2<kBf16>(pr[0], pr[1]));
+          b[blk][n][1] = transposed(pack2<kBf16>(pr[2], pr[3]));
         }
-      }
-      float base[2] = {0.0f, 0.0f}, fade[2] = {1.0f, 1.0f};
-#pragma unroll
-      for (int half = 0; half < 2; half++) {
-        if (half == 1 && !upper) continue;
-        top[half] = quad_max(top[half]);
-        base[half] = top[half] == kNegInf ? 0.0f : top[half];
-        fade[half] = exp2_fast(m_run[half] - base[half]);
-      }
-      if (__any_sync(0xffffffffu, top[0] != m_run[0] || (upper && top[1] != m_run[1]))) {
-#pragma unroll
-        for (int s = 0; s < kSteps; s++)
-#pragma unroll
-          for (int n = 0; n < 2; n++)
-#pragma unroll
-            for (int e = 0; e < 4; e++) acc[s][n][e] *= fade[e >> 1];
-        l_run[0] *= fade[0];
-        l_run[1] *= fade[1];
-        m_run[0] = top[0];
-        if (upper) m_run[1] = top[1];
-      }
-      // ---- probabilities and the weighted sum of values
-      uint32_t a[kBlocks][4];
-#pragma unroll
-      for (int blk = 0; blk < kBlocks; blk++) {
-        float pr[2][4] = {};
-#pragma unroll
-        for (int half = 0; half < 2; half++) {
-          if (half == 1 && !upper) continue;
-#pragma unroll
-          for (int n = 0; n < 2; n++)
-#pragma unroll
-            for (int e = 0; e < 2; e++) {
-              pr[n][2 * half + e] = exp2_fast(sc[blk][n][2 * half + e] - base[half]);
-              l_run[half] += pr[n][2 * half + e];
-            }
-        }
-#pragma unroll
-        for (int n = 0; n < 2; n++) {
-          a[blk][2 * n] = pack2<kBf16>(pr[n][0], pr[n][1]);
-          a[blk][2 * n + 1] = pack2<kBf16>(pr[n][2], pr[n][3]);
-        }
-      }
       if constexpr (!kE4m3) {
 #pragma unroll
         for (int s = 0; s < kSteps; s++)
 #pragma unroll
           for (int blk = 0; blk < kBlocks; blk++) {
-            uint32_t vf[4];   // rows 0-7, 8-15 of columns 0-7, then of columns 8-15
-            ldsm4_t(vf, v_addr + chunk_at<S::kRowBytes>(w0 + blk * 16 + (lane & 15), s * 2 + (lane >> 4)));
-            mma16816<kBf16>(acc[s][0], a[blk], vf[0], vf[1]);
-            mma16816<kBf16>(acc[s][1], a[blk], vf[2], vf[3]);
+            uint32_t a[4];    // transposed: values 0-7, 8-15 of rows 0-7, then of rows 8-15
+            ldsm4_t(a, v_addr + chunk_at<S::kRowBytes>(w0 + blk * 16 + (lane & 7) + ((lane >> 4) << 3), s * 2 + ((lane >> 3) & 1)));
+#pragma unroll
+            for (int n = 0; n < NT; n++) mma16816<kBf16>(acc[s][n], a, b[blk][n][0], b[blk][n][1]);
           }
       } else {
 #pragma unroll
         for (int s = 0; s < kSteps; s += 2)
 #pragma unroll
           for (int blk = 0; blk < kBlocks; blk++) {
-            // transposed 16-bit units: a lane gets columns 2u, 2u + 1 (u = lane / 4) of two rows, byte by byte; the bytes
-            // are dealt out to the products of the even and of the odd columns
+            // transposed 16-bit units: a lane gets values 2u, 2u + 1 (u = lane / 4) of two rows, byte by byte; even
+            // values become rows 0-7 of the product, odd ones rows 8-15
             uint32_t vf[4];
             ldsm4_t(vf, v_addr + chunk_at<S::kRowBytes>(w0 + blk * 16 + (lane & 15), s + (lane >> 4)));
 #pragma unroll
             for (int u = 0; u < 2; u++) {
-              uint32_t even0, even1, odd0, odd1;
-              e4m3_to_f16(__byte_perm(vf[2 * u], 0, 0x3120), even0, odd0);
-              e4m3_to_f16(__byte_perm(vf[2 * u + 1], 0, 0x3120), even1, odd1);
-              mma16816<false>(acc[s + u][0], a[blk], even0, even1);
-              mma16816<false>(acc[s + u][1], a[blk], odd0, odd1);
+              uint32_t a[4];
+              e4m3_to_f16(__byte_perm(vf[2 * u], 0, 0x3120), a[0], a[1]);
+              e4m3_to_f16(__byte_perm(vf[2 * u + 1], 0, 0x3120), a[2], a[3]);
+#pragma unroll
+              for (int n = 0; n < NT; n++) mma16816<false>(acc[s + u][n], a, b[blk][n][0], b[blk][n][1]);
             }
           }
       }
@@ -623,55 +639,49 @@ __global__ void __launch_bounds__(kThreads, Shape<ST, DP, WM>::kMinCtas) attend_
       const bool whole = from_start && to_end;
       const float v_scale = kE4m3 && p.cache.value_scale != nullptr ? __ldg(p.cache.value_scale + head) : 1.0f;
 #pragma unroll
-      for (int half = 0; half < 2; half++) {
-        const float l = quad_sum(l_run[half]);
-        if ((lane & 3) == 0) ml[warp * 16 + half * 8 + (lane >> 2)] = make_float2(m_run[half], l);
-      }
+      for (int n = 0; n < NT; n++)
+#pragma unroll
+        for (int e = 0; e < 2; e++) {
+          const float l = column_sum(l_run[n][e]);
+          if (row == 0) ml[warp * kHeads + n * 8 + col + e] = make_float2(m_run[n][e], l);
+        }
       compute_sync();                                       // every warp is done with this stage's tile
       float* const sums = reinterpret_cast<float*>(smem + stage * 2 * S::kTileBytes);   // [warps][8][DP]
       const int64_t part = (static_cast<int64_t>(blockIdx.x) * 2 + part_slot(range.first, range.first + i - at.j)) * S::kUnitRows;
       const int64_t unit_at = (static_cast<int64_t>(at.b) * units + head * p.chunks + at.chunk) * S::kUnitRows;
 #pragma unroll
-      for (int half = 0; half < 2; half++) {
-        if (half * 8 >= unit_heads) break;                  // (for every warp: rows of wm 0 come first)
-        {
-          const int row = lane >> 2;
+      for (int n = 0; n < NT; n++) {
+        if (n * 8 >= unit_heads) break;                     // (for every warp: heads of wm 0 come first)
+#pragma unroll
+        for (int e = 0; e < 2; e++) {
           float m = kNegInf;
 #pragma unroll
-          for (int x = 0; x < S::kWT; x++) m = fmaxf(m, ml[(x * WM + wm) * 16 + half * 8 + row].x);
-          const float f = exp2_fast(m_run[half] - (m == kNegInf ? 0.0f : m));
-          float* const to = sums + (warp * 8 + row) * DP;
+          for (int x = 0; x < S::kWT; x++) m = fmaxf(m, ml[(x * WM + wm) * kHeads + n * 8 + col + e].x);
+          const float f = exp2_fast(m_run[n][e] - (m == kNegInf ? 0.0f : m));
+          // value v of head h at v ^ 8 (h / 2 mod 4): the lanes of a store fall into different banks
+          float* const to = sums + (warp * 8 + col + e) * DP;
 #pragma unroll
-          for (int s = 0; s < kSteps; s++) {
+          for (int s = 0; s < kSteps; s++)
 #pragma unroll
             for (int x = 0; x < 2; x++) {
-              float2 v;
-              int col;
-              if constexpr (!kE4m3) {
-                v = make_float2(acc[s][x][2 * half] * f, acc[s][x][2 * half + 1] * f);
-                col = s * 16 + x * 8 + (lane & 3) * 2;
-              } else {
-                v = make_float2(acc[s][0][2 * half + x] * f, acc[s][1][2 * half + x] * f);
-                col = s * 16 + (lane & 3) * 4 + x * 2;
-              }
-              *reinterpret_cast<float2*>(to + (col ^ ((row & 3) << 3))) = v;
+              const int v = s * 16 + (kE4m3 ? row * 2 + x : row + x * 8);
+              to[v ^ ((col >> 1) << 3)] = acc[s][n][2 * x + e] * f;
             }
-          }
         }
         compute_sync();
-        // warp w puts out rows w, w + 4, ..
+        // warp w puts out heads w, w + 4, ..
         for (int rr = warp; rr < WM * 8; rr += kComputeWarps) {
-          const int w = rr >> 3, row = rr & 7;
-          const int hr = w * 16 + half * 8 + row;           // query head inside the unit
+          const int w = rr >> 3, h8 = rr & 7;
+          const int hr = w * kHeads + n * 8 + h8;           // query head inside the unit
           if (hr >= unit_heads) continue;
           float m = kNegInf, l = 0.0f;
 #pragma unroll
-          for (int x = 0; x < S::kWT; x++) m = fmaxf(m, ml[(x * WM + w) * 16 + half * 8 + row].x);
-          const float base = m == kNegInf ? 0.0f : m;
+          for (int x = 0; x < S::kWT; x++) m = fmaxf(m, ml[(x * WM + w) * kHeads + n * 8 + h8].x);
+          const float from = m == kNegInf ? 0.0f : m;
 #pragma unroll
           for (int x = 0; x < S::kWT; x++) {
-            const float2 o = ml[(x * WM + w) * 16 + half * 8 + row];
-            l += o.y * exp2_fast(o.x - base);
+            const float2 o = ml[(x * WM + w) * kHeads + n * 8 + h8];
+            l += o.y * exp2_fast(o.x - from);
           }
           const int q_head = head * p.group + unit_first + hr;
           const float inv = l == 0.0f ? 0.0f : v_scale / l;
@@ -681,7 +691,7 @@ __global__ void __launch_bounds__(kThreads, Shape<ST, DP, WM>::kMinCtas) attend_
             if (d >= width) break;
             float v = 0.0f;
 #pragma unroll
-            for (int x = 0; x < S::kWT; x++) v += sums[((x * WM + w) * 8 + row) * DP + (d ^ ((row & 3) << 3))];
+            for (int x = 0; x < S::kWT; x++) v += sums[((x * WM + w) * 8 + h8) * DP + (d ^ ((h8 >> 1) << 3))];
             if (whole) store16(p.out + at.b * p.out_seq + q_head * p.out_head + d * 2, v * inv, p.q_bf16);
             else p.part_acc[(part + hr) * width + d] = v;
           }
@@ -708,7 +718,7 @@ __global__ void __launch_bounds__(kThreads, Shape<ST, DP, WM>::kMinCtas) attend_
   }
 }
 
-template <typename ST, int DP, int WM>
+template <typename ST, int DP, int WM, int NT>
 struct Launcher {
   static void prepare() {
     static std::atomic<uint64_t> done{0};                   // one bit per device
@@ -716,8 +726,8 @@ struct Launcher {
     NVE_B200_CUDA(cudaGetDevice(&dev));
     const uint64_t bit = uint64_t{1} << (dev & 63);
     if (done.load(std::memory_order_acquire) & bit) return;
-    NVE_B200_CUDA(cudaFuncSetAttribute(attend_kernel<ST, DP, WM>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                       Shape<ST, DP, WM>::kSmem));
+    NVE_B200_CUDA(cudaFuncSetAttribute(attend_kernel<ST, DP, WM, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                       Shape<ST, DP, WM, NT>::kSmem));
     done.fetch_or(bit, std::memory_order_acq_rel);
   }
   static int resident() {
@@ -728,35 +738,34 @@ struct Launcher {
     if (n > 0) return n;
     prepare();
     int per_sm = 0;
-    NVE_B200_CUDA(cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, attend_kernel<ST, DP, WM>, kThreads,
-                                                               Shape<ST, DP, WM>::kSmem));
+    NVE_B200_CUDA(cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, attend_kernel<ST, DP, WM, NT>, kThreads,
+                                                               Shape<ST, DP, WM, NT>::kSmem));
     n = std::max(1, per_sm) * sm_count();
     cached[dev & 63].store(n, std::memory_order_release);
     return n;
   }
   static void launch(const KvAttendParams& p, cudaStream_t stream) {
     prepare();
-    attend_kernel<ST, DP, WM><<<p.ctas, kThreads, Shape<ST, DP, WM>::kSmem, stream>>>(p);
+    attend_kernel<ST, DP, WM, NT><<<p.ctas, kThreads, Shape<ST, DP, WM, NT>::kSmem, stream>>>(p);
     NVE_B200_CUDA(cudaGetLastError());
   }
 };
 
-// fn(Launcher<ST, DP, WM>{}) for the variant of this width and number of padded query rows
+// fn(Launcher{}) for the variant of this width and number of padded query rows
+template <typename ST, int DP, typename Fn>
+auto with_rows(int rows_per_unit, Fn&& fn) {
+  if (rows_per_unit == 8) return fn(Launcher<ST, DP, 1, 1>{});
+  if (rows_per_unit == 16) return fn(Launcher<ST, DP, 1, 2>{});
+  if (rows_per_unit == 32) return fn(Launcher<ST, DP, 2, 2>{});
+  return fn(Launcher<ST, DP, 4, 2>{});
+}
 template <typename ST, typename Fn>
 auto with_variant(int width, int rows_per_unit, Fn&& fn) {
-  if (width <= 64) {
-    if (rows_per_unit == 16) return fn(Launcher<ST, 64, 1>{});
-    if (rows_per_unit == 32) return fn(Launcher<ST, 64, 2>{});
-    return fn(Launcher<ST, 64, 4>{});
+  switch (kv_padded_width(width)) {
+    case 64: return with_rows<ST, 64>(rows_per_unit, fn);
+    case 128: return with_rows<ST, 128>(rows_per_unit, fn);
+    default: return with_rows<ST, 256>(rows_per_unit, fn);
   }
-  if (width <= 128) {
-    if (rows_per_unit == 16) return fn(Launcher<ST, 128, 1>{});
-    if (rows_per_unit == 32) return fn(Launcher<ST, 128, 2>{});
-    return fn(Launcher<ST, 128, 4>{});
-  }
-  if (rows_per_unit == 16) return fn(Launcher<ST, 256, 1>{});
-  if (rows_per_unit == 32) return fn(Launcher<ST, 256, 2>{});
-  return fn(Launcher<ST, 256, 4>{});
 }
 
 }  // namespace kv

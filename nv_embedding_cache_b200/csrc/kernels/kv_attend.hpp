@@ -19,7 +19,7 @@ struct KvAttendParams {
   int32_t chunk;                     // query heads one unit takes (group split over `chunks` units)
   int32_t chunks;
   int32_t tile_rows;                 // kv_tile_rows of this width and type
-  int32_t rows_per_unit;             // padded rows of a unit in the scratch: 16, 32 or 64
+  int32_t rows_per_unit;             // padded rows of a unit in the scratch: 8, 16, 32 or 64
   float scale_log2;                  // scale * log2(e)
   // scratch
   float* part_acc;                   // [ctas][2][rows_per_unit][width]

@@ -27,6 +27,13 @@ constexpr int kStep = kThreads * 4;    // rows a weight block takes at once
 constexpr int kMaxChunk = 64;          // query heads of a unit
 constexpr float kNegInf = -__builtin_huge_valf();
 
+// relative error 2^-22; a probability below 2^-126 is 0
+__device__ __forceinline__ float exp2_fast(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
 // The CTAs that had a part of the unit that begins at tile `first_tile`, and where their parts are in the scratch: a
 // CTA's first part is slot 0, and only the first CTA of a unit can have it second.
 struct Parts {
@@ -61,7 +68,7 @@ struct JoinPlan {
   int32_t per_unit;                  // join blocks of a unit
 };
 
-__global__ void __launch_bounds__(kThreads) join_kernel(const KvAttendParams p, const JoinPlan plan) {
+__global__ void __launch_bounds__(kThreads, 3) join_kernel(const KvAttendParams p, const JoinPlan plan) {
   __shared__ int64_t s_sum[kWarps][2];
   __shared__ float s_lse[kMaxChunk];
   __shared__ float s_l[kWarps], s_acc[kWarps][256];
@@ -165,23 +172,18 @@ __global__ void __launch_bounds__(kThreads) join_kernel(const KvAttendParams p, 
   const int slice_end = min(row0 + plan.slice_rows, length);
   // four rows of one page are one piece of memory where pages hold fours
   const bool four = p.cache.page_size % 4 == 0 && reinterpret_cast<uint64_t>(p.cache.weights) % 16 == 0;
-  float* at[4];
-  // where the weights of the four rows from `row` on are; nullptr: not there
-  auto find = [&](int row) {
+  // pages and slots of the four rows from `row` on (with `four`, of the first); page -1: not there
+  auto find = [&](int row, int32_t (&page)[4], int32_t (&slot)[4]) {
 #pragma unroll
     for (int x = 0; x < 4; x++) {
-      at[x] = nullptr;
-      if (row + x >= length) continue;
-      if (x > 0 && four) {
-        at[x] = at[0] == nullptr ? nullptr : at[0] + x;
-        continue;
+      page[x] = -1;
+      if (row + x < slice_end && (x == 0 || !four)) {
+        page[x] = kv_locate(p.cache, p.table.pages, p.table.stride, b, row + x, &slot[x]);
       }
-      int32_t slot;
-      const int32_t page = kv_locate(p.cache, p.table.pages, p.table.stride, b, row + x, &slot);
-      if (page >= 0) at[x] = p.cache.weights + kv_weight_index(p.cache, page, head, slot);
     }
   };
-  find(row0 + tid * 4);
+  int32_t page[4], slot[4];
+  find(row0 + tid * 4, page, slot);
   first_launch_done();
   for (int chunk = 0; chunk < p.chunks; chunk++) {
     const int unit = head * p.chunks + chunk;
@@ -208,31 +210,59 @@ __global__ void __launch_bounds__(kThreads) join_kernel(const KvAttendParams p, 
       }
     }
     __syncthreads();
+    if (chunk > 0) find(row0 + tid * 4, page, slot);
     for (int row = row0 + tid * 4; row < slice_end; row += kStep) {
-      if (chunk > 0 || row >= row0 + kStep) find(row);
-      float4 old = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-      const bool piece = four && at[3] != nullptr;
-      if (piece) old = *reinterpret_cast<const float4*>(at[0]);
+      // in this order, so that nothing waits before everything is under way: scores, weights, the pages of the next step
+      constexpr int kAtOnce = 8;
       const int tile = row / p.tile_rows, in_tile = row % p.tile_rows;
       const float* const s = p.scores + (static_cast<int64_t>(first_tile) + tile) * p.chunk * p.tile_rows + in_tile;
+      float4 x[kAtOnce];
+#pragma unroll
+      for (int g = 0; g < kAtOnce; g++)
+        if (g < heads) x[g] = *reinterpret_cast<const float4*>(s + g * p.tile_rows);
       float w[4] = {};
-#pragma unroll 8
-      for (int g = 0; g < heads; g++) {
-        const float4 x = *reinterpret_cast<const float4*>(s + g * p.tile_rows);
-        const float e = s_lse[g];
-        if (e != kNegInf) {
-          w[0] += exp2f(x.x - e);
-          w[1] += exp2f(x.y - e);
-          w[2] += exp2f(x.z - e);
-          w[3] += exp2f(x.w - e);
+      float* at[4];
+      const bool piece = four && row + 3 < slice_end && page[0] >= 0;
+      if (piece) {
+        at[0] = p.cache.weights + kv_weight_index(p.cache, page[0], head, slot[0]);
+        const float4 old = *reinterpret_cast<const float4*>(at[0]);
+        w[0] = old.x;
+        w[1] = old.y;
+        w[2] = old.z;
+        w[3] = old.w;
+      } else {
+#pragma unroll
+        for (int y = 0; y < 4; y++) {
+          at[y] = nullptr;
+          const int from = four ? 0 : y;
+          if (row + y < slice_end && page[from] >= 0) {
+            at[y] = p.cache.weights + kv_weight_index(p.cache, page[from], head, slot[from]) + (four ? y : 0);
+            w[y] = *at[y];
+          }
+        }
+      }
+      find(row + kStep, page, slot);
+      float sum[4] = {};
+      for (int g0 = 0; g0 < heads; g0 += kAtOnce) {
+#pragma unroll
+        for (int g = 0; g < kAtOnce; g++) {
+          if (g0 + g >= heads) break;
+          if (g0 > 0) x[g] = *reinterpret_cast<const float4*>(s + (g0 + g) * p.tile_rows);
+          const float e = s_lse[g0 + g];
+          if (e != kNegInf) {
+            sum[0] += exp2_fast(x[g].x - e);
+            sum[1] += exp2_fast(x[g].y - e);
+            sum[2] += exp2_fast(x[g].z - e);
+            sum[3] += exp2_fast(x[g].w - e);
+          }
         }
       }
       if (piece) {
-        *reinterpret_cast<float4*>(at[0]) = make_float4(old.x + w[0], old.y + w[1], old.z + w[2], old.w + w[3]);
+        *reinterpret_cast<float4*>(at[0]) = make_float4(w[0] + sum[0], w[1] + sum[1], w[2] + sum[2], w[3] + sum[3]);
       } else {
 #pragma unroll
-        for (int x = 0; x < 4; x++)
-          if (at[x] != nullptr) *at[x] += w[x];
+        for (int y = 0; y < 4; y++)
+          if (at[y] != nullptr) *at[y] = w[y] + sum[y];
       }
     }
   }
@@ -244,9 +274,9 @@ void launch_kv_join(const KvAttendParams& p, int sms, cudaStream_t stream) {
   const int64_t lists = static_cast<int64_t>(p.table.sequences) * p.cache.heads;
   const int64_t unit_count = lists * p.chunks;
   JoinPlan plan{};
-  // slices: four blocks per SM (as many as run at once) if the rows are enough for that
+  // slices: three blocks per SM (as many as run at once) if the rows are enough for that
   const int64_t most = std::max<int64_t>(1, ceil_div(p.table.capacity, kStep));
-  const int64_t wanted = std::min<int64_t>(most, std::max<int64_t>(1, int64_t{4} * sms / lists));
+  const int64_t wanted = std::min<int64_t>(most, std::max<int64_t>(1, int64_t{3} * sms / lists));
   plan.slice_rows = static_cast<int32_t>(ceil_div(most, wanted) * kStep);
   plan.slices = static_cast<int32_t>(std::max<int64_t>(1, ceil_div(p.table.capacity, plan.slice_rows)));
   plan.weight_blocks = p.scores != nullptr ? static_cast<int32_t>(lists * plan.slices) : 0;
