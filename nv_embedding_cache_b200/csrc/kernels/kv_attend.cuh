@@ -183,17 +183,17 @@ __global__ void __launch_bounds__(kThreads, Shape<ST, DP, WM, NT>::kMinCtas) att
     }
   }
   // ---- the number of tiles, and where this CTA's run of them begins
-  __shared__ int64_t s_sum[kThreads / 32];
+  __shared__ int32_t s_sum[kThreads / 32];
   __shared__ int32_t s_start[3];
   {
-    int64_t mine = 0;
+    int32_t mine = 0;
     for (int b = tid; b < p.table.sequences; b += kThreads) mine += tiles_of(kv_length(p.table, b, p.cache.status), S::kTile);
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) mine += __shfl_xor_sync(0xffffffffu, mine, o);
     if (lane == 0) s_sum[warp] = mine;
     __syncthreads();
   }
-  int64_t total = 0;
+  int32_t total = 0;                                        // below 2^31, as the host has seen to
 #pragma unroll
   for (int w = 0; w < kThreads / 32; w++) total += s_sum[w];
   total *= units;
@@ -210,29 +210,30 @@ __global__ void __launch_bounds__(kThreads, Shape<ST, DP, WM, NT>::kMinCtas) att
     }
   }
   if (total == 0) return;
-  const int32_t n_ctas = static_cast<int32_t>(min(static_cast<int64_t>(gridDim.x), total));
-  if (static_cast<int32_t>(blockIdx.x) >= n_ctas) return;
-  const TileRange range = tile_range(total, n_ctas, blockIdx.x);
-  const int n_tiles = range.last - range.first;
+  const int32_t n_ctas = min(static_cast<int32_t>(gridDim.x), total), me = blockIdx.x;
+  if (me >= n_ctas) return;
+  const TileSplit split = tile_split(total, n_ctas);
+  const int32_t first_tile = run_first(split, me);
+  const int n_tiles = run_first(split, me + 1) - first_tile;
 
   if (warp == 0) {                                          // 32 sequences a step
-    int64_t before = 0;
+    int32_t before = 0;
     for (int base = 0; base < p.table.sequences; base += 32) {
       const int b = base + lane;
       const int nt = b < p.table.sequences ? tiles_of(kv_length(p.table, b, nullptr), S::kTile) : 0;
-      const int64_t here = static_cast<int64_t>(nt) * units;
-      int64_t incl = here;
+      const int32_t here = nt * units;
+      int32_t incl = here;
 #pragma unroll
       for (int o = 1; o < 32; o <<= 1) {
-        const int64_t x = __shfl_up_sync(0xffffffffu, incl, o);
+        const int32_t x = __shfl_up_sync(0xffffffffu, incl, o);
         if (lane >= o) incl += x;
       }
-      const int64_t at = range.first - (before + incl - here);
+      const int32_t at = first_tile - (before + incl - here);
       const bool found = at >= 0 && at < here;
       if (found) {
         s_start[0] = b;
-        s_start[1] = static_cast<int32_t>(at) / nt;
-        s_start[2] = static_cast<int32_t>(at) % nt;
+        s_start[1] = at / nt;
+        s_start[2] = at % nt;
       }
       if (__any_sync(0xffffffffu, found)) break;
       before += __shfl_sync(0xffffffffu, incl, 31);
@@ -548,7 +549,7 @@ __global__ void __launch_bounds__(kThreads, Shape<ST, DP, WM, NT>::kMinCtas) att
               if (!((there[blk] >> (row + (e >> 1) * 8)) & 1u)) sc[blk][n][e] = kNegInf;
       }
       if (p.scores != nullptr) {
-        float* const to = p.scores + ((static_cast<int64_t>(range.first) + i) * p.chunk + wm * kHeads + col) * S::kTile + w0 + row;
+        float* const to = p.scores + ((static_cast<int64_t>(first_tile) + i) * p.chunk + wm * kHeads + col) * S::kTile + w0 + row;
 #pragma unroll
         for (int n = 0; n < NT; n++)
 #pragma unroll
@@ -647,7 +648,7 @@ __global__ void __launch_bounds__(kThreads, Shape<ST, DP, WM, NT>::kMinCtas) att
         }
       compute_sync();                                       // every warp is done with this stage's tile
       float* const sums = reinterpret_cast<float*>(smem + stage * 2 * S::kTileBytes);   // [warps][8][DP]
-      const int64_t part = (static_cast<int64_t>(blockIdx.x) * 2 + part_slot(range.first, range.first + i - at.j)) * S::kUnitRows;
+      const int64_t part = (static_cast<int64_t>(blockIdx.x) * 2 + part_slot(first_tile, first_tile + i - at.j)) * S::kUnitRows;
       const int64_t unit_at = (static_cast<int64_t>(at.b) * units + head * p.chunks + at.chunk) * S::kUnitRows;
 #pragma unroll
       for (int n = 0; n < NT; n++) {

@@ -43,11 +43,11 @@ struct Parts {
     return (static_cast<int64_t>(c) * 2 + (c == first ? first_slot : 0)) * p.rows_per_unit;
   }
 };
-__device__ __forceinline__ Parts parts_of(int64_t total, int32_t n, int32_t first_tile, int32_t tiles) {
+__device__ __forceinline__ Parts parts_of(TileSplit split, int32_t first_tile, int32_t tiles) {
   Parts r;
-  r.first = cta_of_tile(total, n, first_tile);
-  r.last = cta_of_tile(total, n, first_tile + tiles - 1);
-  r.first_slot = part_slot(tile_range(total, n, r.first).first, first_tile);
+  r.first = cta_of_tile(split, first_tile);
+  r.last = cta_of_tile(split, first_tile + tiles - 1);
+  r.first_slot = part_slot(run_first(split, r.first), first_tile);
   return r;
 }
 
@@ -69,7 +69,7 @@ struct JoinPlan {
 };
 
 __global__ void __launch_bounds__(kThreads, 3) join_kernel(const KvAttendParams p, const JoinPlan plan) {
-  __shared__ int64_t s_sum[kWarps][2];
+  __shared__ int32_t s_sum[kWarps][2];
   __shared__ float s_lse[kMaxChunk];
   __shared__ float s_l[kWarps], s_acc[kWarps][256];
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
@@ -87,7 +87,7 @@ __global__ void __launch_bounds__(kThreads, 3) join_kernel(const KvAttendParams 
     return;
   }
   // tiles of all sequences, and of those before b
-  int64_t all = 0, before = 0;
+  int32_t all = 0, before = 0;
   for (int x = tid; x < p.table.sequences; x += kThreads) {
     const int nt = tiles_of(kv_length(p.table, x, nullptr), p.tile_rows);
     all += nt;
@@ -109,14 +109,14 @@ __global__ void __launch_bounds__(kThreads, 3) join_kernel(const KvAttendParams 
     all += s_sum[w][0];
     before += s_sum[w][1];
   }
-  const int64_t total = all * units;
-  const int32_t n = static_cast<int32_t>(min(static_cast<int64_t>(p.ctas), total));
-  const int32_t seq_tile = static_cast<int32_t>(before * units);
+  const int32_t total = all * units;                        // below 2^31, as the host has seen to
+  const TileSplit split = tile_split(total, min(p.ctas, total));
+  const int32_t seq_tile = before * units;
 
   if (!weights) {
     // ---- join of some query heads of a unit
     const int unit = list - b * units;
-    const Parts parts = parts_of(total, n, seq_tile + unit * tiles, tiles);
+    const Parts parts = parts_of(split, seq_tile + unit * tiles, tiles);
     first_launch_done();
     if (parts.first == parts.last) return;                  // done by the CTA that had it alone
     const int head = unit / p.chunks, chunk = unit - head * p.chunks;
@@ -189,7 +189,7 @@ __global__ void __launch_bounds__(kThreads, 3) join_kernel(const KvAttendParams 
     const int unit = head * p.chunks + chunk;
     const int32_t first_tile = seq_tile + unit * tiles;
     const int heads = min(p.chunk, p.group - chunk * p.chunk);
-    const Parts parts = parts_of(total, n, first_tile, tiles);
+    const Parts parts = parts_of(split, first_tile, tiles);
     if (chunk > 0) __syncthreads();
     if (parts.first == parts.last) {
       if (tid < heads) s_lse[tid] = p.unit_lse[(static_cast<int64_t>(b) * units + unit) * p.rows_per_unit + tid];

@@ -32,9 +32,10 @@ NVE_KV_FN uint32_t fast_div(uint32_t n, const FastDiv& f) {
 }
 
 // ---- tiles of the attention -----------------------------------------------------------------------
-// Tiles (kv_tile_rows rows of one unit = a key head and a chunk of its query heads) are numbered sequence by sequence, inside
-// a sequence unit by unit, inside a unit along the length.  CTA c of n takes the run [c total / n, (c + 1) total / n):
-// every CTA gets the same number of tiles, give or take one, whatever the lengths are.  n <= total, so no run is empty.
+// Tiles (kv_tile_rows rows of one unit = a key head and a chunk of its query heads) are numbered sequence by sequence,
+// inside a sequence unit by unit, inside a unit along the length.  n CTAs take runs of them in order, the first `more`
+// of `each` + 1 tiles, the others of `each`: the work is the same for all, whatever the lengths are.  n <= total, so no
+// run is empty.
 // Rows of a tile: 16 KB of keys and 16 KB of values for rows of 128 and 256 bytes (the width is padded to 64, 128 or
 // 256 values); 128 rows at most, so that short sequences still make several tiles.
 constexpr int kKvMaxTile = 128;
@@ -47,18 +48,18 @@ NVE_KV_FN int32_t tiles_of(int32_t length, int32_t tile_rows) {   // a power of 
   return static_cast<int32_t>((static_cast<uint32_t>(length) + tile_rows - 1) / static_cast<uint32_t>(tile_rows));
 }
 
-struct TileRange {
-  int32_t first, last;
+struct TileSplit {
+  int32_t each, more;
 };
-NVE_KV_FN TileRange tile_range(int64_t total, int32_t n, int32_t c) {
-  return {static_cast<int32_t>(total * c / n), static_cast<int32_t>(total * (c + 1) / n)};
-}
-// The CTA whose run holds tile t: the largest c with c total < (t + 1) n.
-NVE_KV_FN int32_t cta_of_tile(int64_t total, int32_t n, int32_t t) {
-  return static_cast<int32_t>(((static_cast<int64_t>(t) + 1) * n - 1) / total);
+NVE_KV_FN TileSplit tile_split(int32_t total, int32_t n) { return {total / n, total % n}; }
+NVE_KV_FN int32_t run_first(TileSplit s, int32_t c) { return c * s.each + (c < s.more ? c : s.more); }
+// The CTA whose run holds tile t.
+NVE_KV_FN int32_t cta_of_tile(TileSplit s, int32_t t) {
+  const int32_t longer = s.more * (s.each + 1);              // tiles of the longer runs
+  return t < longer ? t / (s.each + 1) : s.more + (t - longer) / s.each;
 }
 // A CTA leaves at most two unfinished units: the one its run begins in and the one it ends in.  Slot of the unit that
-// begins at tile `unit_first` in the scratch of a CTA whose run begins at `run_first`.
-NVE_KV_FN int32_t part_slot(int32_t run_first, int32_t unit_first) { return run_first >= unit_first ? 0 : 1; }
+// begins at tile `unit_first` in the scratch of a CTA whose run begins at tile `first`.
+NVE_KV_FN int32_t part_slot(int32_t first, int32_t unit_first) { return first >= unit_first ? 0 : 1; }
 
 }  // namespace nve_b200
