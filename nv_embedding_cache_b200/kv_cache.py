@@ -18,16 +18,20 @@ import ctypes as C
 import math
 
 import torch
-from torch.autograd.function import once_differentiable
 
 from . import capi
 
+_E4M3 = torch.float8_e4m3fn
 _DTYPES = {torch.float32: capi.DTYPE_FLOAT32, torch.float16: capi.DTYPE_FLOAT16, torch.bfloat16: capi.DTYPE_BFLOAT16,
-           torch.float8_e4m3fn: capi.DTYPE_E4M3}
+           _E4M3: capi.DTYPE_E4M3}
+_INT32 = torch.int32
 _raw_stream = torch._C._cuda_getCurrentRawStream
+_current_device = torch._C._cuda_getDevice
+_GROUPS = (None, capi.HeadRows * 1, capi.HeadRows * 2)
 
 
 def _need(ok: bool, message: str) -> None:
+    """For checks outside the calls of a decode step; those spell their messages out only when they fail."""
     if not ok:
         raise ValueError(message)
 
@@ -35,7 +39,7 @@ def _need(ok: bool, message: str) -> None:
 def _call(fn, device: torch.device, *args) -> None:
     """fn(*args, stream) on `device` and its current stream."""
     index = device.index
-    if torch.cuda.current_device() == index:
+    if _current_device() == index:
         status = fn(*args, _raw_stream(index))
     else:
         with torch.cuda.device(index):
@@ -45,9 +49,10 @@ def _call(fn, device: torch.device, *args) -> None:
 
 
 def _int32(t: torch.Tensor, device: torch.device, dims: int, name: str) -> torch.Tensor:
-    _need(t.dtype == torch.int32 and t.device == device and t.dim() == dims,
-          f"{name} must be an int32 tensor with {dims} dimension(s) on {device}")
-    _need(t.stride(-1) == 1 or t.shape[-1] <= 1, f"the last dimension of {name} must be dense")
+    if t.dtype is not _INT32 or t.device != device or t.dim() != dims:
+        raise ValueError(f"{name} must be an int32 tensor with {dims} dimension(s) on {device}")
+    if t.stride(-1) != 1 and t.shape[-1] > 1:
+        raise ValueError(f"the last dimension of {name} must be dense")
     return t
 
 
@@ -58,10 +63,11 @@ def _rows(t: torch.Tensor) -> torch.Tensor:
 
 def _head_rows(t: torch.Tensor, out) -> capi.HeadRows:
     e = t.element_size()
+    s = t.stride()
     if out is None:
-        return capi.HeadRows(t.data_ptr(), None, t.stride(0) * e, t.stride(1) * e, 0, 0, t.shape[1])
-    return capi.HeadRows(t.data_ptr(), out.data_ptr(), t.stride(0) * e, t.stride(1) * e, out.stride(0) * e,
-                         out.stride(1) * e, t.shape[1])
+        return capi.HeadRows(t.data_ptr(), None, s[0] * e, s[1] * e, 0, 0, t.shape[1])
+    o = out.stride()
+    return capi.HeadRows(t.data_ptr(), out.data_ptr(), s[0] * e, s[1] * e, o[0] * e, o[1] * e, t.shape[1])
 
 
 class RotaryPlan:
@@ -85,6 +91,8 @@ class RotaryPlan:
         self.num_pairs, self.num_axes, self.interleaved = inv_freq.numel(), num_axes, bool(interleaved)
         self.device = inv_freq.device
         self.status = torch.zeros(1, dtype=torch.int32, device=self.device)
+        self._constant = (inv_freq.data_ptr(), None if pair_axis is None else pair_axis.data_ptr(), self.num_pairs,
+                          int(self.interleaved), self.status.data_ptr())
 
     @classmethod
     def sections(cls, pairs_per_axis, *, base: float = 10000.0, restart: bool = False, interleaved: bool = False,
@@ -108,59 +116,72 @@ class RotaryPlan:
             raise RuntimeError("rotary plan: an entry of pair_axis is not in [0, num_axes)")
 
     def _args(self, positions: torch.Tensor, tokens: int, device: torch.device) -> capi.Rotary:
-        _need(positions.dtype == torch.int32 and positions.device == device == self.device,
-              f"positions must be int32 and, like the plan, on {device}")
+        if positions.dtype is not _INT32 or positions.device != device or device != self.device:
+            raise ValueError(f"positions must be int32 and, like the plan, on {device}")
         if positions.dim() == 1:
             positions = positions[None]
-        _need(positions.dim() == 2 and positions.shape[0] == self.num_axes and positions.shape[1] == tokens,
-              f"positions must be [{self.num_axes}, {tokens}]")
-        return capi.Rotary(positions.data_ptr(), positions.stride(0), positions.stride(1), self.num_axes,
-                           self.inv_freq.data_ptr(), None if self.pair_axis is None else self.pair_axis.data_ptr(),
-                           self.num_pairs, self.interleaved, self.status.data_ptr())
+        if tuple(positions.shape) != (self.num_axes, tokens):
+            raise ValueError(f"positions must be [{self.num_axes}, {tokens}]")
+        s = positions.stride()
+        return capi.Rotary(positions.data_ptr(), s[0], s[1], self.num_axes, *self._constant)
 
 
 def _turn(plan: RotaryPlan, positions: torch.Tensor, tensors, backward: bool):
     """New tensors with the rows of `tensors` ([tokens, heads, width] each) turned."""
-    outs = [torch.empty(t.shape, dtype=t.dtype, device=t.device) for t in tensors]
+    tensors = [_rows(t) for t in tensors]
+    outs = [torch.empty_like(t) for t in tensors]
     first = tensors[0]
-    groups = (capi.HeadRows * len(outs))(*[_head_rows(t, o) for t, o in zip(tensors, outs)])
-    args = plan._args(positions, first.shape[0], first.device)
-    _call(capi.lib.nve_b200_rotary, first.device, C.byref(args), _DTYPES[first.dtype], first.shape[2], first.shape[0],
-          groups, len(outs), backward)
+    shape = first.shape
+    groups = _GROUPS[len(outs)](*map(_head_rows, tensors, outs))
+    _call(capi.lib.nve_b200_rotary, first.device, plan._args(positions, shape[0], first.device), _DTYPES[first.dtype],
+          shape[2], shape[0], groups, len(outs), backward)
     return outs
 
 
 class _RotaryFunction(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, plan, positions, *tensors):
-        ctx.plan = plan
-        ctx.set_materialize_grads(False)
-        ctx.save_for_backward(positions, plan.inv_freq, plan.pair_axis)
-        return tuple(_turn(plan, positions, [_rows(t) for t in tensors], False))
+    """The rotation is linear in its rows and its transpose is the rotation by the negated angles, so the gradient is
+    the same function again (and has a gradient in turn)."""
 
     @staticmethod
-    @once_differentiable
+    def forward(ctx, plan, positions, backward, *tensors):
+        ctx.plan, ctx.turned_back = plan, backward
+        ctx.set_materialize_grads(False)
+        ctx.save_for_backward(positions)
+        return tuple(_turn(plan, positions, tensors, backward))
+
+    @staticmethod
     def backward(ctx, *grads):
-        positions = ctx.saved_tensors[0]
-        at = [i for i, g in enumerate(grads) if g is not None and ctx.needs_input_grad[2 + i]]
+        positions, = ctx.saved_tensors
         out = [None] * len(grads)
+        at = [i for i, g in enumerate(grads) if g is not None and ctx.needs_input_grad[3 + i]]
         if at:
-            for i, g in zip(at, _turn(ctx.plan, positions, [_rows(grads[i]) for i in at], True)):
+            taken = [grads[i] for i in at]
+            if torch.is_grad_enabled():
+                turned = _RotaryFunction.apply(ctx.plan, positions, not ctx.turned_back, *taken)
+            else:
+                turned = _turn(ctx.plan, positions, taken, not ctx.turned_back)
+            for i, g in zip(at, turned):
                 out[i] = g
-        return (None, None, *out)
+        return (None, None, None, *out)
 
 
 def rotary(q: torch.Tensor, k: torch.Tensor | None, positions: torch.Tensor, plan: RotaryPlan):
     """Queries and keys ([tokens, heads, width], fp32, fp16 or bf16) turned by their positions ([axes, tokens] int32).
-    Returns new tensors (q', k'), q' alone when `k` is None.  Differentiable in q and k."""
+    Returns new tensors (q', k'), q' alone when `k` is None.  Differentiable in q and k, any number of times."""
     tensors = (q,) if k is None else (q, k)
-    for t in tensors:
-        _need(t.is_cuda and t.dim() == 3, "q and k must be [tokens, heads, width] on the GPU")
-        _need(t.dtype in _DTYPES and t.dtype != torch.float8_e4m3fn, "q and k must be fp32, fp16 or bf16")
-        _need(t.dtype == q.dtype and t.device == q.device and t.shape[0] == q.shape[0] and t.shape[2] == q.shape[2],
-              "q and k must agree in type, device, tokens and width")
-    out = _RotaryFunction.apply(plan, positions, *tensors)
-    return out[0] if k is None else out
+    shape, dtype, device = q.shape, q.dtype, q.device
+    if not q.is_cuda or len(shape) != 3:
+        raise ValueError("q and k must be [tokens, heads, width] on the GPU")
+    if dtype not in _DTYPES or dtype is _E4M3:
+        raise ValueError("q and k must be fp32, fp16 or bf16")
+    if k is not None and (k.dtype is not dtype or k.device != device or k.dim() != 3 or k.shape[0] != shape[0]
+                          or k.shape[2] != shape[2]):
+        raise ValueError("q and k must agree in type, device, tokens and width")
+    if torch.is_grad_enabled() and (q.requires_grad or (k is not None and k.requires_grad)):
+        out = _RotaryFunction.apply(plan, positions, False, *tensors)
+    else:
+        out = _turn(plan, positions, tensors, False)
+    return out[0] if k is None else tuple(out)
 
 
 class PagedKVCache:
@@ -202,7 +223,6 @@ class PagedKVCache:
         self._view = capi.KvCache(keys.data_ptr(), values.data_ptr(), strides(keys), strides(values), address(weights),
                                   address(key_scale), address(value_scale), _DTYPES[keys.dtype], pages, size, heads,
                                   width, self.status.data_ptr())
-        self._ref = C.byref(self._view)
         self._scratch_sizes = {}
 
     @classmethod
@@ -229,16 +249,19 @@ class PagedKVCache:
     def _table(self, page_table: torch.Tensor, lengths: torch.Tensor) -> int:
         _int32(page_table, self.device, 2, "page_table")
         _int32(lengths, self.device, 1, "lengths")
-        _need(lengths.shape[0] == page_table.shape[0], "page_table and lengths must have one row per sequence")
-        return page_table.shape[0]
+        n = page_table.shape[0]
+        if lengths.shape[0] != n:
+            raise ValueError("page_table and lengths must have one row per sequence")
+        return n
 
     def _row_dtype(self, t: torch.Tensor, name: str) -> int:
-        _need(t.device == self.device and t.dim() == 3 and t.shape[2] == self.head_width,
-              f"{name} must be [.., heads, {self.head_width}] on {self.device}")
-        _need(t.dtype == self.dtype or (self.dtype == torch.float8_e4m3fn and t.dtype in (torch.float16, torch.bfloat16)),
-              f"{name} must have the cache's type, or fp16 or bf16 for an E4M3 cache")
-        _need(t.dtype != torch.float8_e4m3fn, f"{name} must be fp16 or bf16")
-        return _DTYPES[t.dtype]
+        if t.device != self.device or t.dim() != 3 or t.shape[2] != self.head_width:
+            raise ValueError(f"{name} must be [.., heads, {self.head_width}] on {self.device}")
+        dtype = t.dtype
+        if dtype is _E4M3 or (dtype is not self.dtype and (self.dtype is not _E4M3 or dtype not in _DTYPES
+                                                           or dtype is torch.float32)):
+            raise ValueError(f"{name} must have the cache's type, or fp16 or bf16 for an E4M3 cache")
+        return _DTYPES[dtype]
 
     def append(self, k: torch.Tensor, v: torch.Tensor, page_table: torch.Tensor, lengths: torch.Tensor, *,
                q: torch.Tensor | None = None, offsets: torch.Tensor | None = None,
@@ -251,28 +274,31 @@ class PagedKVCache:
         n = self._table(page_table, lengths)
         dtype = self._row_dtype(k, "k")
         tokens = k.shape[0]
-        self._row_dtype(v, "v")
-        _need(v.dtype == k.dtype and v.shape == k.shape and k.shape[1] == self.num_heads,
-              "k and v must agree and have the cache's heads")
+        if v.dtype is not k.dtype or v.shape != k.shape or v.device != self.device or k.shape[1] != self.num_heads:
+            raise ValueError("k and v must agree and have the cache's heads")
         k, v = _rows(k), _rows(v)
         turned = None
-        q_rows = capi.HeadRows()
-        if q is not None:
+        if q is None:
+            q_rows = capi.HeadRows()
+        else:
             self._row_dtype(q, "q")
-            _need(q.dtype == k.dtype and q.shape[0] == tokens, "q must have the type and the tokens of k")
+            if q.dtype is not k.dtype or q.shape[0] != tokens:
+                raise ValueError("q must have the type and the tokens of k")
             q = _rows(q)
-            turned = torch.empty(q.shape, dtype=q.dtype, device=self.device)
+            turned = torch.empty_like(q)
             q_rows = _head_rows(q, turned)
         if offsets is not None:
             _int32(offsets, self.device, 1, "offsets")
-            _need(offsets.shape[0] == n + 1, "offsets must have one entry more than there are sequences")
-        _need((rotary is None) == (positions is None), "positions and rotary go together")
+            if offsets.shape[0] != n + 1:
+                raise ValueError("offsets must have one entry more than there are sequences")
+        if (rotary is None) != (positions is None):
+            raise ValueError("positions and rotary go together")
         turn = None if rotary is None else C.pointer(rotary._args(positions, tokens, self.device))
-        new_lengths = torch.empty(n, dtype=torch.int32, device=self.device)
+        new_lengths = torch.empty_like(lengths, memory_format=torch.contiguous_format)
         args = capi.KvAppend(dtype, tokens, q_rows, _head_rows(k, None), _head_rows(v, None), turn,
                              page_table.data_ptr(), page_table.stride(0), page_table.shape[1], n, lengths.data_ptr(),
                              None if offsets is None else offsets.data_ptr(), new_lengths.data_ptr(), 1)
-        _call(capi.lib.nve_b200_kv_append, self.device, self._ref, C.byref(args))
+        _call(capi.lib.nve_b200_kv_append, self.device, self._view, args)
         return turned, new_lengths
 
     def attend(self, q: torch.Tensor, page_table: torch.Tensor, lengths: torch.Tensor, *, scale: float | None = None,
@@ -284,33 +310,35 @@ class PagedKVCache:
         with it the scratch; ``accumulate_weights`` adds each row's probabilities to ``weights``."""
         n = self._table(page_table, lengths)
         dtype = self._row_dtype(q, "q")
-        heads = q.shape[1]
-        _need(q.shape[0] == n, "q must have one row per sequence")
-        rows = page_table.shape[1] * self.page_size
+        if q.shape[0] != n:
+            raise ValueError("q must have one row per sequence")
+        heads, width, device = q.shape[1], self.head_width, self.device
+        pages = page_table.shape[1]
         if max_length is None:
-            max_length = rows
+            max_length = pages * self.page_size
         q = _rows(q)
         e = q.element_size()
-        if q.data_ptr() % 16 or q.stride(0) * e % 16 or q.stride(1) * e % 16:
+        s = q.stride()
+        if q.data_ptr() % 16 or s[0] * e % 16 or s[1] * e % 16:
             q = q.clone(memory_format=torch.contiguous_format)
-        out = torch.empty((n, heads, self.head_width), dtype=q.dtype, device=self.device)
-        lse = torch.empty((n, heads), dtype=torch.float32, device=self.device) if return_lse else None
-        args = capi.KvAttend(dtype, n, heads, q.data_ptr(), q.stride(0) * e, q.stride(1) * e, out.data_ptr(),
-                             heads * self.head_width * e, self.head_width * e, None if lse is None else lse.data_ptr(),
-                             page_table.data_ptr(), page_table.stride(0), page_table.shape[1], lengths.data_ptr(),
-                             max_length, 1.0 / math.sqrt(self.head_width) if scale is None else scale,
-                             accumulate_weights)
+            s = q.stride()
+        out = torch.empty((n, heads, width), dtype=q.dtype, device=device)
+        lse = torch.empty((n, heads), dtype=torch.float32, device=device) if return_lse else None
+        args = capi.KvAttend(dtype, n, heads, q.data_ptr(), s[0] * e, s[1] * e, out.data_ptr(), heads * width * e,
+                             width * e, None if lse is None else lse.data_ptr(), page_table.data_ptr(),
+                             page_table.stride(0), pages, lengths.data_ptr(), max_length,
+                             1.0 / math.sqrt(width) if scale is None else scale, accumulate_weights)
         key = (n, heads, max_length, accumulate_weights)
         size = self._scratch_sizes.get(key)
         if size is None:
             size = C.c_size_t()
-            _call(capi.lib.nve_b200_kv_attend, self.device, self._ref, C.byref(args), None, C.byref(size))
+            _call(capi.lib.nve_b200_kv_attend, device, self._view, args, None, size)
             if len(self._scratch_sizes) >= 4096:
                 self._scratch_sizes.clear()
             self._scratch_sizes[key] = size
         if n:
-            scratch = torch.empty(size.value, dtype=torch.uint8, device=self.device)
-            _call(capi.lib.nve_b200_kv_attend, self.device, self._ref, C.byref(args), scratch.data_ptr(), C.byref(size))
+            scratch = torch.empty(size.value, dtype=torch.uint8, device=device)
+            _call(capi.lib.nve_b200_kv_attend, device, self._view, args, scratch.data_ptr(), size)
         return (out, lse) if return_lse else out
 
     def evict(self, page_table: torch.Tensor, lengths: torch.Tensor, new_page_table: torch.Tensor, budget: int, *,
@@ -322,14 +350,17 @@ class PagedKVCache:
         the old row of each new one, -1 behind the last; new lengths)."""
         n = self._table(page_table, lengths)
         _int32(new_page_table, self.device, 2, "new_page_table")
-        _need(new_page_table.shape[0] == n, "new_page_table must have one row per sequence")
-        _need(budget > 0, "budget must be positive")
+        if new_page_table.shape[0] != n:
+            raise ValueError("new_page_table must have one row per sequence")
+        if budget <= 0:
+            raise ValueError("budget must be positive")
+        pages = page_table.shape[1]
         if max_length is None:
-            max_length = page_table.shape[1] * self.page_size
-        kept = torch.empty((n, self.num_heads, budget), dtype=torch.int32, device=self.device)
-        new_lengths = torch.empty(n, dtype=torch.int32, device=self.device)
-        args = capi.KvEvict(n, page_table.data_ptr(), page_table.stride(0), page_table.shape[1], lengths.data_ptr(),
-                            max_length, new_page_table.data_ptr(), new_page_table.stride(0), new_page_table.shape[1],
-                            budget, sinks, recent, kept.data_ptr(), new_lengths.data_ptr())
-        _call(capi.lib.nve_b200_kv_evict, self.device, self._ref, C.byref(args))
+            max_length = pages * self.page_size
+        kept = torch.empty((n, self.num_heads, budget), dtype=_INT32, device=self.device)
+        new_lengths = torch.empty_like(lengths, memory_format=torch.contiguous_format)
+        args = capi.KvEvict(n, page_table.data_ptr(), page_table.stride(0), pages, lengths.data_ptr(), max_length,
+                            new_page_table.data_ptr(), new_page_table.stride(0), new_page_table.shape[1], budget, sinks,
+                            recent, kept.data_ptr(), new_lengths.data_ptr())
+        _call(capi.lib.nve_b200_kv_evict, self.device, self._view, args)
         return kept, new_lengths
