@@ -1,13 +1,15 @@
 // Eviction from the paged cache by accumulated weight: choose the rows that stay, then move them.
 //
 // Choosing, for every (sequence, head): the `budget` largest weights, equal ones by index.  A thread-block cluster
-// takes one list, its CTAs equal runs of it.  The weights become unsigned keys in the same order (rows that must
-// stay the largest of all) and stay in shared memory; a radix select over digits of 11, 11 and 10 bits finds the key of the last
-// row that stays: every CTA counts its run, the counts are added up in the first CTA's shared memory (DSMEM), which finds
-// the digit.  A second pass turns ballots into places in ascending order.  No sort, no scratch in memory, the weights
-// are read once: 4 bytes per row and head.  Latency bounds it (three rounds of counting and cluster barriers).
+// takes one list, its CTAs equal runs of it.  The weights become unsigned keys in the same order (rows that must stay
+// the largest of all) and stay in shared memory; a radix select over digits of 11, 11 and 10 bits finds the key of
+// the last row that stays: every CTA counts the digits of its run, then every CTA adds up all CTAs' counts over
+// DSMEM and finds the digit for itself, which takes one cluster barrier a digit.  Then ballots become places in
+// ascending order.  No sort, no scratch in memory, the weights are read once: 4 bytes per row and head.  Latency bounds
+// it (a chain of page lookup, weights, three rounds of counting, places).
 //
-// Moving: rows of 2 width values per kept row and head, read from anywhere, written page after page; HBM bounds it.
+// Moving: rows of 2 width values per kept row and head, read from anywhere, written page after page; HBM bounds it.  A
+// warp looks up sixteen rows, a lane each, and copies them without a barrier.
 #include <algorithm>
 #include <atomic>
 
@@ -22,28 +24,30 @@ namespace {
 
 namespace cg = cooperative_groups;
 
-constexpr int kThreads = 512;
+constexpr int kThreads = 1024;
 constexpr int kWarps = kThreads / 32;
 constexpr int kBins = 2048;
+constexpr int kEach = kBins / kThreads;    // digits a thread looks after
 constexpr int kMaxCluster = 8;
 constexpr int kMaxCached = 40 * 1024;      // keys one CTA keeps in shared memory
 constexpr uint32_t kMustStay = 0xffffffffu;
+constexpr uint32_t kZero = 0x80000000u;    // key of a row that never drew any attention
 constexpr uint32_t kLowest = 0x007fffffu;  // key of -inf
 
 // Larger weight, larger key; +0 and -0 alike; NaN as -inf.
 __device__ __forceinline__ uint32_t weight_key(float w) {
   if (w != w) return kLowest;
-  if (w == 0.0f) return 0x80000000u;
+  if (w == 0.0f) return kZero;
   const uint32_t u = __float_as_uint(w);
   return (u & 0x80000000u) ? ~u : (u | 0x80000000u);
 }
 
 template <bool CACHED>
 __global__ void __launch_bounds__(kThreads) select_kernel(const KvEvictParams p) {
-  extern __shared__ uint32_t cached[];
-  __shared__ uint32_t hist[kBins];
+  extern __shared__ __align__(16) uint32_t cached[];
+  __shared__ __align__(16) uint32_t hist[2][kBins];
   __shared__ uint32_t s_warp[kWarps][2];
-  __shared__ uint32_t s_found[2];          // in the first CTA: digit, rows of larger digits
+  __shared__ uint32_t s_found[2];          // digit, rows of larger digits
   __shared__ uint32_t s_counts[2];         // of this CTA: keys above the limit, keys at it
   cg::cluster_group cluster = cg::this_cluster();
   const int ranks = static_cast<int>(cluster.num_blocks()), rank = static_cast<int>(cluster.block_rank());
@@ -63,75 +67,98 @@ __global__ void __launch_bounds__(kThreads) select_kernel(const KvEvictParams p)
   // runs of whole warps' steps
   const int step = ((length + ranks - 1) / ranks + 31) & ~31;
   const int first = min(rank * step, length), last = min(first + step, length);
+  const int fixed_end = length - p.recent;
   auto load_key = [&](int i) -> uint32_t {
-    if (i < p.sinks || i >= length - p.recent) return kMustStay;
+    if (i < p.sinks || i >= fixed_end) return kMustStay;
     int32_t slot;
     const int32_t page = kv_locate(p.cache, p.table.pages, p.table.stride, b, i, &slot);
     return page < 0 ? kLowest : weight_key(p.cache.weights[kv_weight_index(p.cache, page, h, slot)]);
   };
   auto key_at = [&](int i) -> uint32_t { return CACHED ? cached[i - first] : load_key(i); };
+  for (int i = tid; i < kBins; i += kThreads) hist[0][i] = hist[1][i] = 0;
+  if (CACHED) {
+    // four rows of a page at once where pages hold fours (runs begin at multiples of 32)
+    if (p.cache.page_size % 4 == 0 && reinterpret_cast<uint64_t>(p.cache.weights) % 16 == 0) {
+#pragma unroll 4
+      for (int i = first + tid * 4; i < last; i += kThreads * 4) {
+        int32_t slot;
+        const int32_t page = kv_locate(p.cache, p.table.pages, p.table.stride, b, i, &slot);
+        float4 w = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        if (page >= 0) w = *reinterpret_cast<const float4*>(p.cache.weights + kv_weight_index(p.cache, page, h, slot));
+        const float v[4] = {w.x, w.y, w.z, w.w};
+        uint32_t k[4];
+#pragma unroll
+        for (int x = 0; x < 4; x++)
+          k[x] = i + x < p.sinks || i + x >= fixed_end ? kMustStay : (page < 0 ? kLowest : weight_key(v[x]));
+        *reinterpret_cast<uint4*>(cached + (i - first)) = make_uint4(k[0], k[1], k[2], k[3]);
+      }
+    } else {
+#pragma unroll 4
+      for (int i = first + tid; i < last; i += kThreads) cached[i - first] = load_key(i);
+    }
+  }
+  __syncthreads();
 
   uint32_t prefix = 0;                     // digits found so far
-  uint32_t need = static_cast<uint32_t>(p.budget);   // rows still to take among keys with this prefix
+  // rows still to take among keys with this prefix; those that must stay are not counted
+  uint32_t need = static_cast<uint32_t>(p.budget - p.sinks - p.recent);
 #pragma unroll 1
-  for (int pass = 0; pass < 3; pass++) {
+  for (int pass = 0; pass < 3 && need > 0; pass++) {
     const int shift = pass == 0 ? 21 : (pass == 1 ? 10 : 0);
     const uint32_t bins = pass == 2 ? 1024u : 2048u;
-    for (int i = tid; i < kBins; i += kThreads) hist[i] = 0;
-    __syncthreads();
-#pragma unroll 4
-    for (int i = first + tid; i < last; i += kThreads) {
-      uint32_t k;
-      if (CACHED && pass == 0) {
-        k = load_key(i);
-        cached[i - first] = k;
-      } else {
-        k = key_at(i);
-      }
-      const bool mine = pass == 0 || (k >> (pass == 1 ? 21 : 10)) == prefix;
-      if (mine) atomicAdd(&hist[(k >> shift) & (bins - 1)], 1u);
-    }
-    cluster.sync();
-    if (rank != 0) {
-      uint32_t* const sum = cluster.map_shared_rank(hist, 0);
-      for (int i = tid; i < static_cast<int>(bins); i += kThreads)
-        if (hist[i] != 0) atomicAdd(sum + i, hist[i]);
-    }
-    cluster.sync();
-    if (rank == 0) {
-      // largest digit d with (rows of digits >= d) >= need
-      constexpr int kEach = kBins / kThreads;
-      uint32_t mine[kEach], own = 0;
-#pragma unroll
-      for (int x = 0; x < kEach; x++) {    // thread 0 has the largest digits
-        const int d = kBins - 1 - (tid * kEach + x);
-        mine[x] = hist[d];
-        own += mine[x];
-      }
-      uint32_t incl = own;
-#pragma unroll
-      for (int o = 1; o < 32; o <<= 1) {
-        const uint32_t x = __shfl_up_sync(0xffffffffu, incl, o);
-        if (lane >= o) incl += x;
-      }
-      if (lane == 31) s_warp[warp][0] = incl;
+    uint32_t* const mine = hist[pass & 1];
+    if (pass == 2) {                       // every CTA is past the barrier after which none reads the first counts
+      for (int i = tid; i < kBins; i += kThreads) mine[i] = 0;
       __syncthreads();
-      uint32_t above = incl - own;
-      for (int w = 0; w < warp; w++) above += s_warp[w][0];
-#pragma unroll
-      for (int x = 0; x < kEach; x++) {
-        if (above < need && above + mine[x] >= need) {
-          s_found[0] = static_cast<uint32_t>(kBins - 1 - (tid * kEach + x));
-          s_found[1] = above;
-        }
-        above += mine[x];
+    }
+    for (int i0 = first; i0 < last; i0 += kThreads) {
+      const int i = i0 + tid;
+      const uint32_t k = i < last ? key_at(i) : kMustStay;
+      const bool counts = k != kMustStay && (pass == 0 || (k >> (pass == 1 ? 21 : 10)) == prefix);
+      // rows that never drew any attention are many and alike: one addition a warp
+      const uint32_t zeros = __ballot_sync(0xffffffffu, counts && k == kZero);
+      if (counts && (k != kZero || lane == __ffs(zeros) - 1)) {
+        atomicAdd(&mine[(k >> shift) & (bins - 1)], k == kZero ? static_cast<uint32_t>(__popc(zeros)) : 1u);
       }
     }
     cluster.sync();
-    const uint32_t* const found = cluster.map_shared_rank(s_found, 0);
-    prefix = (prefix << (pass == 2 ? 10 : 11)) | found[0];
-    need -= found[1];
+    // largest digit d with (rows of digits >= d) >= need; thread 0 has the largest digits
+    const int lowest = kBins - (tid + 1) * kEach;
+    uint32_t sum[kEach] = {};
+    for (int r = 0; r < ranks; r++) {
+      const uint2 x = *reinterpret_cast<const uint2*>(cluster.map_shared_rank(mine, r) + lowest);
+      sum[0] += x.x;
+      sum[1] += x.y;
+    }
+    uint32_t incl = sum[0] + sum[1];
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const uint32_t x = __shfl_up_sync(0xffffffffu, incl, o);
+      if (lane >= o) incl += x;
+    }
+    if (lane == 31) s_warp[warp][0] = incl;
+    __syncthreads();
+    uint32_t above = incl - sum[0] - sum[1];
+    {
+      uint32_t x = lane < warp ? s_warp[lane][0] : 0;
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1) x += __shfl_xor_sync(0xffffffffu, x, o);
+      above += x;
+    }
+#pragma unroll
+    for (int x = kEach - 1; x >= 0; x--) {
+      if (above < need && above + sum[x] >= need) {
+        s_found[0] = static_cast<uint32_t>(lowest + x);
+        s_found[1] = above;
+      }
+      above += sum[x];
+    }
+    __syncthreads();
+    prefix = (prefix << (pass == 2 ? 10 : 11)) | s_found[0];
+    need -= s_found[1];
+    __syncthreads();
   }
+  if (p.budget == p.sinks + p.recent) prefix = kMustStay - 1;   // nothing else stays
   // keys above `prefix` stay, of those equal to it the first `need`
   const int per_warp = ((last - first + kWarps - 1) / kWarps + 31) & ~31;
   const int w_first = min(first + warp * per_warp, last), w_last = min(w_first + per_warp, last);
@@ -178,45 +205,55 @@ __global__ void __launch_bounds__(kThreads) select_kernel(const KvEvictParams p)
 }
 
 constexpr int kMoveThreads = 256;
-constexpr int kMoveRows = 32;
+constexpr int kMoveRows = 16;                               // rows a warp moves
+constexpr int kMoveBlockRows = kMoveRows * kMoveThreads / 32;
 
 __global__ void __launch_bounds__(kMoveThreads) move_kernel(const KvEvictParams p, int32_t blocks_per_list,
                                                             FastDiv chunk_div) {
-  __shared__ int64_t src[2][kMoveRows], dst[2][kMoveRows];
-  const int list = blockIdx.x / blocks_per_list, j0 = (blockIdx.x - list * blocks_per_list) * kMoveRows;
+  const int list = blockIdx.x / blocks_per_list;
   const int b = list / p.cache.heads, h = list - b * p.cache.heads;
+  const int lane = threadIdx.x & 31;
+  const int j0 = (blockIdx.x - list * blocks_per_list) * kMoveBlockRows + (threadIdx.x >> 5) * kMoveRows;
   const int count = min(kv_length(p.table, b, nullptr), p.budget);
-  if (j0 >= count) return;
   const int rows = min(kMoveRows, count - j0);
-  if (static_cast<int>(threadIdx.x) < rows) {
-    const int j = j0 + threadIdx.x;
+  if (rows <= 0) return;                                    // the whole warp
+  // lanes 0-15 look up the keys of a row, lanes 16-31 its values
+  const bool values = lane >= kMoveRows;
+  const int mine = lane & (kMoveRows - 1);
+  const uint8_t* src = nullptr;
+  uint8_t* dst = nullptr;
+  if (mine < rows) {
+    const int j = j0 + mine;
     const int32_t from = p.kept[static_cast<int64_t>(list) * p.budget + j];
     int32_t s_slot, d_slot;
     const int32_t sp = kv_locate(p.cache, p.table.pages, p.table.stride, b, from, &s_slot);
     const int32_t dp = kv_locate(p.cache, p.new_pages, p.new_stride, b, j, &d_slot);
-    const bool ok = sp >= 0 && dp >= 0;
-    src[0][threadIdx.x] = ok ? sp * p.cache.k_page + s_slot * p.cache.k_slot + h * p.cache.k_head : -1;
-    src[1][threadIdx.x] = sp * p.cache.v_page + s_slot * p.cache.v_slot + h * p.cache.v_head;
-    dst[0][threadIdx.x] = dp * p.cache.k_page + d_slot * p.cache.k_slot + h * p.cache.k_head;
-    dst[1][threadIdx.x] = dp * p.cache.v_page + d_slot * p.cache.v_slot + h * p.cache.v_head;
-    if (ok) p.cache.weights[kv_weight_index(p.cache, dp, h, d_slot)] = p.cache.weights[kv_weight_index(p.cache, sp, h, s_slot)];
+    if (sp >= 0 && dp >= 0) {
+      const int64_t page = values ? p.cache.v_page : p.cache.k_page, slot = values ? p.cache.v_slot : p.cache.k_slot;
+      uint8_t* const pool = (values ? p.cache.values : p.cache.keys) + h * (values ? p.cache.v_head : p.cache.k_head);
+      src = pool + sp * page + s_slot * slot;
+      dst = pool + dp * page + d_slot * slot;
+      if (!values) p.cache.weights[kv_weight_index(p.cache, dp, h, d_slot)] = p.cache.weights[kv_weight_index(p.cache, sp, h, s_slot)];
+    }
   }
-  __syncthreads();
-  const int chunks = p.row_bytes / 16, work = rows * 2 * chunks;   // keys of a row, then its values
+  // keys and values of the rows: 2 * rows lines of `chunks` 16-byte pieces, line 2 r + 1 the values of row r
+  const int chunks = p.row_bytes / 16, work = rows * 2 * chunks;
   constexpr int U = 4;
-  for (int w0 = threadIdx.x; w0 < work; w0 += kMoveThreads * U) {
+  for (int w0 = 0; w0 < work; w0 += 32 * U) {
     uint4 x[U];
     uint8_t* to[U];
 #pragma unroll
     for (int u = 0; u < U; u++) {
-      const int w = w0 + u * kMoveThreads;
+      const int w = w0 + u * 32 + lane;
+      const int line = static_cast<int>(fast_div(w, chunk_div)), c = w - line * chunks;
+      const int owner = ((line >> 1) & (kMoveRows - 1)) + (line & 1) * kMoveRows;
+      const uint64_t s = __shfl_sync(0xffffffffu, reinterpret_cast<uint64_t>(src), owner);
+      const uint64_t d = __shfl_sync(0xffffffffu, reinterpret_cast<uint64_t>(dst), owner);
       to[u] = nullptr;
-      if (w >= work) continue;
-      const int r2 = static_cast<int>(fast_div(w, chunk_div)), c = w - r2 * chunks;
-      const int r = r2 >> 1, kv = r2 & 1;
-      if (src[0][r] < 0) continue;
-      x[u] = *reinterpret_cast<const uint4*>((kv ? p.cache.values : p.cache.keys) + src[kv][r] + c * 16);
-      to[u] = (kv ? p.cache.values : p.cache.keys) + dst[kv][r] + c * 16;
+      if (w < work && s != 0) {
+        x[u] = *reinterpret_cast<const uint4*>(s + c * 16);
+        to[u] = reinterpret_cast<uint8_t*>(d + c * 16);
+      }
     }
 #pragma unroll
     for (int u = 0; u < U; u++)
@@ -264,7 +301,7 @@ void launch_kv_evict(const KvEvictParams& p, int sms, cudaStream_t stream) {
   else launch_select<false>(p, ranks, 0, stream);
   const int32_t most = std::min(p.budget, p.table.capacity);
   if (most == 0) return;
-  const int32_t per_list = static_cast<int32_t>(ceil_div(most, kMoveRows));
+  const int32_t per_list = static_cast<int32_t>(ceil_div(most, kMoveBlockRows));
   move_kernel<<<static_cast<unsigned>(lists * per_list), kMoveThreads, 0, stream>>>(
       p, per_list, make_fast_div(static_cast<uint32_t>(p.row_bytes / 16)));
   NVE_B200_CUDA(cudaGetLastError());

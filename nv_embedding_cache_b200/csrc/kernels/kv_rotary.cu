@@ -2,9 +2,10 @@
 //
 // (a, b) -> (a cos - b sin, b cos + a sin) with angle = positions[axis of the pair][token] * inv_freq[pair].
 // Every value is read once and written once and meets three flops, so memory bounds it.  The angles are shared by
-// all heads of a token: a block takes a few whole tokens, computes their cosines and sines once into shared memory
-// and then streams the rows of every head past them, one 16-byte vector (two for the split pairing: the vector of
-// the a's and that of the b's) per thread and step.  The queries, keys and values of a token go through one launch.
+// all heads of a token: a block takes a few whole tokens and computes their cosines and sines once into shared memory.
+// A thread then keeps those of one item (a 16-byte vector of the row, or two for the split pairing: the vector of
+// the a's and that of the b's) in registers and walks over the rows of several heads, the next row's load always under
+// way; the first one's starts before the angles.  The queries, keys and values of a token go through one launch.
 //
 // The angle is the product of a 32-bit integer and an fp32 number: exact in 64 bits up to its last two bits.  It is
 // reduced there (in turns, so that the reduction is a subtraction of an integer) and only the remainder is
@@ -52,12 +53,21 @@ __device__ __forceinline__ void store_vec(uint8_t* p, const float (&x)[VEC]) {
   *reinterpret_cast<Vec<T, VEC>*>(p) = u;
 }
 
-// Stored value of an E4M3 cache: x / scale, rounded to nearest even, saturated to the largest finite value.
+// Stored value of an E4M3 cache: x / scale, rounded to nearest even, saturated to the largest finite value.  One
+// division per row: x (1 / scale) rounds once more, 2^-24, against the 2^-4 of the stored value.
 template <int VEC>
-__device__ __forceinline__ void store_e4m3(uint8_t* p, const float (&x)[VEC], float scale) {
+__device__ __forceinline__ void store_e4m3(uint8_t* p, const float (&x)[VEC], float inverse) {
   Vec<uint8_t, VEC> u;
+  if constexpr (VEC == 1) {
+    u.v[0] = __nv_cvt_float_to_fp8(x[0] * inverse, __NV_SATFINITE, __NV_E4M3);
+  } else {
 #pragma unroll
-  for (int i = 0; i < VEC; i++) u.v[i] = __nv_cvt_float_to_fp8(x[i] / scale, __NV_SATFINITE, __NV_E4M3);
+    for (int i = 0; i < VEC; i += 2) {
+      const __nv_fp8x2_storage_t two = __nv_cvt_float2_to_fp8x2(make_float2(x[i] * inverse, x[i + 1] * inverse), __NV_SATFINITE, __NV_E4M3);
+      u.v[i] = static_cast<uint8_t>(two & 0xff);
+      u.v[i + 1] = static_cast<uint8_t>(two >> 8);
+    }
+  }
   *reinterpret_cast<Vec<uint8_t, VEC>*>(p) = u;
 }
 
@@ -68,18 +78,24 @@ struct TokenPlace {
   bool padding;                     // belongs to no sequence: nothing of it is written
 };
 
-// Which sequence a token belongs to and where its row goes.
+// Which sequence token t belongs to and where its row goes; found by a whole warp, 32 offsets a step.
 __device__ __forceinline__ TokenPlace place_token(const RotaryParams& p, int32_t t) {
   TokenPlace r{0, 0, 0, false, true};
+  const int lane = threadIdx.x & 31;
   int32_t b, first;
   if (p.offsets != nullptr) {
+    // lo: the last sequence that begins at or before t.  Offsets that do not ascend give some sequence; the row is
+    // checked below whatever it is.
     const int32_t n = p.table.sequences;
     if (t < __ldg(p.offsets) || t >= __ldg(p.offsets + n)) return r;
-    int32_t lo = 0, hi = n;         // offsets[lo] <= t < offsets[hi]
-    while (hi - lo > 1) {
-      const int32_t mid = (lo + hi) >> 1;
-      if (__ldg(p.offsets + mid) <= t) lo = mid;
-      else hi = mid;
+    int32_t lo = 0, span = n;
+    while (span > 1) {
+      const int32_t stride = (span + 31) / 32;
+      const int32_t at = lo + lane * stride;
+      const bool before = lane * stride < span && __ldg(p.offsets + at) <= t;
+      const int32_t steps = 31 - __clz(__ballot_sync(0xffffffffu, before) | 1u);
+      lo += steps * stride;
+      span = min(stride, span - steps * stride);
     }
     b = lo;
     first = __ldg(p.offsets + lo);
@@ -105,26 +121,64 @@ __device__ __forceinline__ TokenPlace place_token(const RotaryParams& p, int32_t
 
 // VEC: values of one vector (16 bytes of T, or 1 where alignment or an odd pair count asks for it).
 template <typename T, int VEC, bool INTERLEAVED, bool TO_CACHE, bool E4M3>
-__global__ void __launch_bounds__(kThreads) rotary_kernel(const RotaryParams p) {
+__global__ void __launch_bounds__(kThreads, 4) rotary_kernel(const RotaryParams p) {
   extern __shared__ float2 turn[];                       // [tokens of the block][pairs] (cos, sin)
   __shared__ TokenPlace place[TO_CACHE ? kMaxTokensPerBlock : 1];
+  constexpr bool kTwo = !INTERLEAVED || VEC == 1;        // the a's and the b's of a turned item are two vectors
+  constexpr int kPairs = kTwo ? VEC : VEC / 2;           // pairs of an item
+  using V = Vec<T, VEC>;
   const int32_t t0 = blockIdx.x * p.tokens_per_block;
   const int32_t nt = min(p.tokens_per_block, p.tokens - t0);
 
+  // this thread: item `item` of the rows r0, r0 + row_lanes, .. of the tokens t, t + token_lanes, ..
+  const int32_t group = threadIdx.x / p.lanes, t_first = group / p.row_lanes, r_first = group - t_first * p.row_lanes;
+  int32_t item = threadIdx.x - group * p.lanes;
+  int32_t t = t_first, r = r_first;
+  bool pair_item, two;
+  int32_t first;
+  const int32_t gap = INTERLEAVED ? 1 : p.pairs;         // from the a's to the b's
+  V a, b;
+  auto set_item = [&]() {
+    pair_item = item < p.turned_items;
+    two = kTwo && pair_item;
+    first = pair_item ? (INTERLEAVED && VEC == 1 ? 2 * item : item * VEC) : 2 * p.pairs + (item - p.turned_items) * VEC;
+  };
+  // group of rows r belongs to: 0 queries, 1 keys, 2 values; r becomes the head
+  auto split_row = [&](int32_t& head) -> int {
+    if (head < p.g[0].heads) return 0;
+    head -= p.g[0].heads;
+    if (head < p.g[1].heads) return 1;
+    head -= p.g[1].heads;
+    return 2;
+  };
+  auto load = [&](int32_t token, int32_t head, V& x, V& y) {
+    const int which = split_row(head);
+    const RowGroup& g = which == 0 ? p.g[0] : (which == 1 ? p.g[1] : p.g[2]);
+    const uint8_t* const src = g.in + (t0 + token) * g.in_token + head * g.in_head + first * static_cast<int64_t>(sizeof(T));
+    x = *reinterpret_cast<const V*>(src);
+    if (two) y = *reinterpret_cast<const V*>(src + gap * static_cast<int64_t>(sizeof(T)));
+  };
+  set_item();
+  const bool works = t < nt && item < p.items;
+  if (works) load(t, r, a, b);
+
   if constexpr (TO_CACHE) {
-    for (int32_t b = blockIdx.x * kThreads + threadIdx.x; b < p.table.sequences; b += gridDim.x * kThreads) {
-      const int32_t more = p.offsets != nullptr ? __ldg(p.offsets + b + 1) - __ldg(p.offsets + b) : p.per_sequence;
-      const int64_t n = static_cast<int64_t>(kv_length(p.table, b, p.cache.status)) + max(more, 0);
-      p.new_lengths[b] = static_cast<int32_t>(min(n, static_cast<int64_t>(p.table.capacity)));
+    for (int32_t s = blockIdx.x * kThreads + threadIdx.x; s < p.table.sequences; s += gridDim.x * kThreads) {
+      const int32_t more = p.offsets != nullptr ? __ldg(p.offsets + s + 1) - __ldg(p.offsets + s) : p.per_sequence;
+      const int64_t n = static_cast<int64_t>(kv_length(p.table, s, p.cache.status)) + max(more, 0);
+      p.new_lengths[s] = static_cast<int32_t>(min(n, static_cast<int64_t>(p.table.capacity)));
     }
-    if (static_cast<int32_t>(threadIdx.x) < nt) place[threadIdx.x] = place_token(p, t0 + threadIdx.x);
+    for (int32_t i = threadIdx.x >> 5; i < nt; i += kThreads / 32) {
+      const TokenPlace at = place_token(p, t0 + i);
+      if ((threadIdx.x & 31) == 0) place[i] = at;
+    }
   }
   for (int32_t i = threadIdx.x; i < nt * p.pairs; i += kThreads) {
-    const int32_t t = i / p.pairs, k = i - t * p.pairs;
+    const int32_t token = i / p.pairs, k = i - token * p.pairs;
     const int32_t axis = p.pair_axis != nullptr ? __ldg(p.pair_axis + k) : 0;
     float2 cs = make_float2(1.0f, 0.0f);
     if (static_cast<uint32_t>(axis) < static_cast<uint32_t>(p.axes)) {
-      const int32_t pos = __ldg(p.positions + axis * p.axis_stride + (t0 + t) * p.token_stride);
+      const int32_t pos = __ldg(p.positions + axis * p.axis_stride + (t0 + token) * p.token_stride);
       const double half_turns = static_cast<double>(pos) * static_cast<double>(__ldg(p.inv_freq + k)) *
                                 0.31830988618379067153776752674503;     // 1 / pi
       const double rest = half_turns - 2.0 * rint(0.5 * half_turns);     // in [-1, 1]
@@ -137,103 +191,91 @@ __global__ void __launch_bounds__(kThreads) rotary_kernel(const RotaryParams p) 
   }
   __syncthreads();
 
-  constexpr bool kTwo = !INTERLEAVED || VEC == 1;        // the a's and the b's of a turned item are two vectors
-  constexpr int U = 2;                                   // items in flight per thread
-  using V = Vec<T, VEC>;
-  const int32_t work = nt * p.rows * p.items;
-  for (int32_t w0 = threadIdx.x; w0 < work; w0 += kThreads * U) {
-    V a[U], b[U];
-    uint8_t* dst[U];
-    int32_t first[U], cs_at[U];                          // cs_at < 0: copied
-    float scale[U];
-    int to[U];                                           // 0: nothing, 1: rows of T, 2: E4M3 rows
-#pragma unroll
-    for (int u = 0; u < U; u++) {
-      const int32_t w = w0 + u * kThreads;
-      to[u] = 0;
-      if (w >= work) continue;
-      const int32_t tr = static_cast<int32_t>(fast_div(w, p.item_div));
-      const int32_t item = w - tr * p.items;
-      const int32_t t = static_cast<int32_t>(fast_div(tr, p.row_div));
-      int32_t head = tr - t * p.rows;
-      const bool is_q = head < p.g[0].heads;
-      if (!is_q) head -= p.g[0].heads;
-      const bool is_v = !is_q && head >= p.g[1].heads;
-      if (is_v) head -= p.g[1].heads;
-      const RowGroup& g = is_q ? p.g[0] : (is_v ? p.g[2] : p.g[1]);
-      const bool pair_item = item < p.turned_items;
-      first[u] = pair_item ? (INTERLEAVED && VEC == 1 ? 2 * item : item * VEC)
-                           : 2 * p.pairs + (item - p.turned_items) * VEC;
-      const int64_t src = (t0 + t) * g.in_token + head * g.in_head + first[u] * static_cast<int64_t>(sizeof(T));
-      if (TO_CACHE && !is_q) {
-        const TokenPlace& at = place[t];
-        if (!at.stored) continue;
-        dst[u] = is_v ? p.cache.values + at.value + head * p.cache.v_head : p.cache.keys + at.key + head * p.cache.k_head;
-        to[u] = E4M3 ? 2 : 1;
-        if constexpr (E4M3) {
-          const float* s = is_v ? p.cache.value_scale : p.cache.key_scale;
-          scale[u] = s != nullptr ? __ldg(s + head) : 1.0f;
-        }
-      } else {
-        dst[u] = g.out + (t0 + t) * g.out_token + head * g.out_head;
-        to[u] = 1;
-        if (TO_CACHE && place[t].padding) {
-          if (!p.zero_padding) {
-            to[u] = 0;
-            continue;
-          }
-          a[u] = b[u] = V{};
-          cs_at[u] = pair_item ? -2 : -1;
-          continue;
-        }
-      }
-      cs_at[u] = pair_item ? (is_v ? -2 : t * p.pairs + (kTwo ? item * VEC : item * (VEC / 2))) : -1;
-      a[u] = *reinterpret_cast<const V*>(g.in + src);
-      if (kTwo && pair_item) {
-        b[u] = *reinterpret_cast<const V*>(g.in + src + (INTERLEAVED ? 1 : p.pairs) * static_cast<int64_t>(sizeof(T)));
+  auto finish = [&](int32_t token, int32_t head, const float2 (&cs)[kPairs], V x_raw, V y_raw) {
+    const int which = split_row(head);
+    bool as_is = which == 2 || !pair_item;
+    uint8_t* dst;
+    if (TO_CACHE && which > 0) {
+      const TokenPlace& at = place[token];
+      if (!at.stored) return;
+      dst = which == 2 ? p.cache.values + at.value + head * p.cache.v_head : p.cache.keys + at.key + head * p.cache.k_head;
+    } else {
+      const RowGroup& g = which == 0 ? p.g[0] : p.g[1];
+      dst = g.out + (t0 + token) * g.out_token + head * g.out_head;
+      if (TO_CACHE && place[token].padding) {
+        if (!p.zero_padding) return;
+        x_raw = y_raw = V{};
+        as_is = true;
       }
     }
+    const bool to_e4m3 = E4M3 && which > 0;
+    if (as_is && !to_e4m3) {
+      *reinterpret_cast<V*>(dst + first * sizeof(T)) = x_raw;
+      if (two) *reinterpret_cast<V*>(dst + (first + gap) * sizeof(T)) = y_raw;
+      return;
+    }
+    float x[VEC], y[VEC];
 #pragma unroll
-    for (int u = 0; u < U; u++) {
-      if (to[u] == 0) continue;
-      const bool two = kTwo && cs_at[u] != -1;
-      const int32_t second = first[u] + (INTERLEAVED ? 1 : p.pairs);
-      if (cs_at[u] < 0 && to[u] == 1) {                  // bytes as they are
-        *reinterpret_cast<V*>(dst[u] + first[u] * sizeof(T)) = a[u];
-        if (two) *reinterpret_cast<V*>(dst[u] + second * sizeof(T)) = b[u];
-        continue;
+    for (int i = 0; i < VEC; i++) {
+      x[i] = Wide<T>::up(x_raw.v[i]);
+      if (kTwo) y[i] = two ? Wide<T>::up(y_raw.v[i]) : 0.0f;
+    }
+    if (!as_is) {
+#pragma unroll
+      for (int i = 0; i < kPairs; i++) {
+        float& xa = kTwo ? x[i] : x[2 * i];
+        float& xb = kTwo ? y[i] : x[2 * i + 1];
+        const float u0 = xa;
+        xa = u0 * cs[i].x - xb * cs[i].y;
+        xb = xb * cs[i].x + u0 * cs[i].y;
       }
-      float x[VEC], y[VEC];
-#pragma unroll
-      for (int i = 0; i < VEC; i++) {
-        x[i] = Wide<T>::up(a[u].v[i]);
-        if (kTwo) y[i] = two ? Wide<T>::up(b[u].v[i]) : 0.0f;
-      }
-      if (cs_at[u] >= 0) {
-        if constexpr (kTwo) {
-#pragma unroll
-          for (int i = 0; i < VEC; i++) {
-            const float2 cs = turn[cs_at[u] + i];
-            const float xa = x[i];
-            x[i] = xa * cs.x - y[i] * cs.y;
-            y[i] = y[i] * cs.x + xa * cs.y;
-          }
-        } else {
-#pragma unroll
-          for (int i = 0; i < VEC / 2; i++) {
-            const float2 cs = turn[cs_at[u] + i];
-            const float xa = x[2 * i];
-            x[2 * i] = xa * cs.x - x[2 * i + 1] * cs.y;
-            x[2 * i + 1] = x[2 * i + 1] * cs.x + xa * cs.y;
-          }
+    }
+    if (to_e4m3) {
+      const float* const s = which == 2 ? p.cache.value_scale : p.cache.key_scale;
+      const float inverse = s != nullptr ? 1.0f / __ldg(s + head) : 1.0f;
+      store_e4m3<VEC>(dst + first, x, inverse);
+      if (two) store_e4m3<VEC>(dst + first + gap, y, inverse);
+    } else {
+      store_vec<T, VEC>(dst + first * sizeof(T), x);
+      if (two) store_vec<T, VEC>(dst + (first + gap) * sizeof(T), y);
+    }
+  };
+
+  if (works) {
+    const int32_t token_lanes = kThreads / p.lanes / p.row_lanes;
+    float2 cs[kPairs];
+    int32_t cs_token = -1, cs_item = -1;
+    for (;;) {
+      // the row after this one: next row, next token, next item
+      int32_t r_next = r + p.row_lanes, t_next = t, item_next = item;
+      if (r_next >= p.rows) {
+        r_next = r_first;
+        t_next += token_lanes;
+        if (t_next >= nt) {
+          t_next = t_first;
+          item_next += p.lanes;
         }
       }
-      if (E4M3 && to[u] == 2) {
-        store_e4m3<VEC>(dst[u] + first[u], x, scale[u]);
-        if (two) store_e4m3<VEC>(dst[u] + second, y, scale[u]);
+      const bool more = item_next < p.items, same_item = item_next == item;
+      V a_next, b_next;
+      if (more && same_item) load(t_next, r_next, a_next, b_next);
+      if (cs_token != t || cs_item != item) {
+#pragma unroll
+        for (int i = 0; i < kPairs; i++) cs[i] = pair_item ? turn[t * p.pairs + item * kPairs + i] : make_float2(1.0f, 0.0f);
+        cs_token = t;
+        cs_item = item;
+      }
+      finish(t, r, cs, a, b);
+      if (!more) break;
+      r = r_next;
+      t = t_next;
+      if (same_item) {
+        a = a_next;
+        b = b_next;
       } else {
-        store_vec<T, VEC>(dst[u] + first[u] * sizeof(T), x);
-        if (two) store_vec<T, VEC>(dst[u] + second * sizeof(T), y);
+        item = item_next;
+        set_item();
+        load(t, r, a, b);
       }
     }
   }
@@ -280,12 +322,15 @@ void launch_type(RotaryParams& p, bool e4m3, bool interleaved, int sms, cudaStre
   const int vec = wide ? W : 1;
   p.turned_items = interleaved && wide ? 2 * p.pairs / vec : p.pairs / vec;
   p.items = p.turned_items + (p.width - 2 * p.pairs) / vec;
-  p.item_div = make_fast_div(static_cast<uint32_t>(p.items));
-  p.row_div = make_fast_div(static_cast<uint32_t>(p.rows));
-  // one token per block until every SM has its eight blocks, then several, so that a block's angles are one step
-  // of all its threads
-  const int64_t fill = static_cast<int64_t>(sms) * 8;
-  p.tokens_per_block = static_cast<int32_t>(std::min<int64_t>(4, std::max<int64_t>(1, p.tokens / fill)));
+  // Threads of a block: `lanes` along the items of a row, then `row_lanes` along the rows of a token, then tokens.  Where
+  // tokens are few, a block is one token and as many rows at once as fit; else a thread walks over about five rows of
+  // a token, and of two tokens where that leaves every SM its blocks twice.
+  p.lanes = std::min(p.items, kThreads);
+  const int32_t groups = kThreads / p.lanes;
+  const bool few = p.tokens < static_cast<int64_t>(sms) * 8;
+  p.row_lanes = std::min({groups, p.rows, few ? groups : static_cast<int32_t>(ceil_div(p.rows, 5))});
+  p.tokens_per_block = few ? 1 : std::min(groups / p.row_lanes, kMaxTokensPerBlock / 2);
+  if (p.tokens / (p.tokens_per_block * 2) >= static_cast<int64_t>(sms) * 8) p.tokens_per_block *= 2;
   if (wide) {
     if (interleaved) launch_dest<T, W, true>(p, e4m3, stream);
     else launch_dest<T, W, false>(p, e4m3, stream);

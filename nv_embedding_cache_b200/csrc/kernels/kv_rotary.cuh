@@ -29,7 +29,8 @@ struct RotaryParams {
   int32_t items;                    // work items of one row
   int32_t turned_items;             // the first of them hold pairs, the others are copied
   int32_t tokens_per_block;
-  FastDiv item_div, row_div;
+  int32_t lanes;                    // threads that share the items of a row
+  int32_t row_lanes;                // threads that share the rows of a token, for one item
   // append
   bool to_cache;
   bool zero_padding;                // queries of padding tokens become zeros
