@@ -3,13 +3,18 @@
 // Choosing, for every (sequence, head): the `budget` largest weights, equal ones by index.  A thread-block cluster
 // takes one list, its CTAs equal runs of it.  The weights become unsigned keys in the same order (rows that must stay
 // the largest of all) and stay in shared memory; a radix select over digits of 11, 11 and 10 bits finds the key of
-// the last row that stays: every CTA counts the digits of its run, then every CTA adds up all CTAs' counts over
-// DSMEM and finds the digit for itself, which takes one cluster barrier a digit.  Then ballots become places in
-// ascending order.  No sort, no scratch in memory, the weights are read once: 4 bytes per row and head.  Latency bounds
+// the last row that stays: every CTA counts the digits of its run, and after one cluster barrier a digit a warp of
+// every CTA finds it for itself from all CTAs' counts, read over DSMEM: first among 64 sums of 32 digits, then among
+// those 32 (reading all 2048 counts of eight CTAs took three times as long).  Then ballots become places in ascending
+// order.  No sort, no scratch in memory, the weights are read once: 4 bytes per row and head.  Latency bounds
 // it (a chain of page lookup, weights, three rounds of counting, places).
 //
-// Moving: rows of 2 width values per kept row and head, read from anywhere, written page after page; HBM bounds it.  A
-// warp looks up sixteen rows, a lane each, and copies them without a barrier.
+// Moving: rows of 2 width values per kept row and head, read from anywhere, written page after page; HBM bounds it.
+// Small blocks, many per SM: a block looks its rows up, a thread each, and copies them with four 16-byte pieces of a
+// thread in flight.  Warps that do both for themselves, or look the next rows up while they copy, keep fewer loads in
+// flight and took 60 and 69 us where this takes 48 (32 lists of 8192 rows of 256 bytes: 5.6 TB/s).
+// The launch overlaps the end of the choosing one (programmatic dependent launch): new pages are looked up before the
+// wait.
 #include <algorithm>
 #include <atomic>
 
@@ -24,10 +29,7 @@ namespace {
 
 namespace cg = cooperative_groups;
 
-constexpr int kThreads = 1024;
-constexpr int kWarps = kThreads / 32;
 constexpr int kBins = 2048;
-constexpr int kEach = kBins / kThreads;    // digits a thread looks after
 constexpr int kMaxCluster = 8;
 constexpr int kMaxCached = 40 * 1024;      // keys one CTA keeps in shared memory
 constexpr uint32_t kMustStay = 0xffffffffu;
@@ -42,18 +44,21 @@ __device__ __forceinline__ uint32_t weight_key(float w) {
   return (u & 0x80000000u) ? ~u : (u | 0x80000000u);
 }
 
-template <bool CACHED>
+template <bool CACHED, int kThreads>
 __global__ void __launch_bounds__(kThreads) select_kernel(const KvEvictParams p) {
+  constexpr int kWarps = kThreads / 32;
   extern __shared__ __align__(16) uint32_t cached[];
   __shared__ __align__(16) uint32_t hist[2][kBins];
+  __shared__ uint32_t coarse[2][64];       // sums of 32 counts
   __shared__ uint32_t s_warp[kWarps][2];
-  __shared__ uint32_t s_found[2];          // digit, rows of larger digits
+  __shared__ uint32_t s_found[3];          // digit, rows of larger digits, rows of this digit
   __shared__ uint32_t s_counts[2];         // of this CTA: keys above the limit, keys at it
   cg::cluster_group cluster = cg::this_cluster();
   const int ranks = static_cast<int>(cluster.num_blocks()), rank = static_cast<int>(cluster.block_rank());
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int list = blockIdx.x / ranks;     // (sequence, head)
   const int b = list / p.cache.heads, h = list - b * p.cache.heads;
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   const int length = kv_length(p.table, b, p.cache.status);
   const int count = min(length, p.budget);
   int32_t* const kept = p.kept + static_cast<int64_t>(list) * p.budget;
@@ -73,6 +78,10 @@ __global__ void __launch_bounds__(kThreads) select_kernel(const KvEvictParams p)
     int32_t slot;
     const int32_t page = kv_locate(p.cache, p.table.pages, p.table.stride, b, i, &slot);
     return page < 0 ? kLowest : weight_key(p.cache.weights[kv_weight_index(p.cache, page, h, slot)]);
+  };
+  auto all_sync = [&]() {
+    if (ranks > 1) cluster.sync();
+    else __syncthreads();
   };
   auto key_at = [&](int i) -> uint32_t { return CACHED ? cached[i - first] : load_key(i); };
   for (int i = tid; i < kBins; i += kThreads) hist[0][i] = hist[1][i] = 0;
@@ -100,6 +109,7 @@ __global__ void __launch_bounds__(kThreads) select_kernel(const KvEvictParams p)
   __syncthreads();
 
   uint32_t prefix = 0;                     // digits found so far
+  bool decided = false;
   // rows still to take among keys with this prefix; those that must stay are not counted
   uint32_t need = static_cast<uint32_t>(p.budget - p.sinks - p.recent);
 #pragma unroll 1
@@ -121,44 +131,76 @@ __global__ void __launch_bounds__(kThreads) select_kernel(const KvEvictParams p)
         atomicAdd(&mine[(k >> shift) & (bins - 1)], k == kZero ? static_cast<uint32_t>(__popc(zeros)) : 1u);
       }
     }
-    cluster.sync();
-    // largest digit d with (rows of digits >= d) >= need; thread 0 has the largest digits
-    const int lowest = kBins - (tid + 1) * kEach;
-    uint32_t sum[kEach] = {};
-    for (int r = 0; r < ranks; r++) {
-      const uint2 x = *reinterpret_cast<const uint2*>(cluster.map_shared_rank(mine, r) + lowest);
-      sum[0] += x.x;
-      sum[1] += x.y;
-    }
-    uint32_t incl = sum[0] + sum[1];
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const uint32_t x = __shfl_up_sync(0xffffffffu, incl, o);
-      if (lane >= o) incl += x;
-    }
-    if (lane == 31) s_warp[warp][0] = incl;
     __syncthreads();
-    uint32_t above = incl - sum[0] - sum[1];
-    {
-      uint32_t x = lane < warp ? s_warp[lane][0] : 0;
+    for (int c = warp; c < 64; c += kWarps) {
+      uint32_t x = mine[c * 32 + lane];
 #pragma unroll
       for (int o = 16; o > 0; o >>= 1) x += __shfl_xor_sync(0xffffffffu, x, o);
-      above += x;
+      if (lane == 0) coarse[pass & 1][c] = x;
     }
+    all_sync();
+    // largest digit d with (rows of digits >= d) >= need; lane 0 has the largest digits
+    if (warp == 0) {
+      uint32_t hi = 0, lo = 0;
+      if (ranks == 1) {
+        hi = coarse[pass & 1][63 - 2 * lane];
+        lo = coarse[pass & 1][62 - 2 * lane];
+      } else {
 #pragma unroll
-    for (int x = kEach - 1; x >= 0; x--) {
-      if (above < need && above + sum[x] >= need) {
-        s_found[0] = static_cast<uint32_t>(lowest + x);
-        s_found[1] = above;
+        for (int r = 0; r < kMaxCluster; r++) {
+          if (r < ranks) {
+            const uint32_t* const theirs = cluster.map_shared_rank(coarse[pass & 1], r);
+            hi += theirs[63 - 2 * lane];
+            lo += theirs[62 - 2 * lane];
+          }
+        }
       }
-      above += sum[x];
+      const auto before = [&](uint32_t x) {                 // sum over the lanes before this one
+        uint32_t incl = x;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+          const uint32_t y = __shfl_up_sync(0xffffffffu, incl, o);
+          if (lane >= o) incl += y;
+        }
+        return incl - x;
+      };
+      uint32_t above = before(hi + lo);
+      const bool in_hi = above < need && above + hi >= need;
+      const bool in_lo = above + hi < need && above + hi + lo >= need;
+      if (in_lo) above += hi;
+      const int src = __ffs(__ballot_sync(0xffffffffu, in_hi || in_lo)) - 1;
+      const int c = __shfl_sync(0xffffffffu, in_hi ? 63 - 2 * lane : 62 - 2 * lane, src);
+      above = __shfl_sync(0xffffffffu, above, src);
+      const int digit = c * 32 + 31 - lane;
+      uint32_t x = 0;
+      if (ranks == 1) {
+        x = mine[digit];
+      } else {
+#pragma unroll
+        for (int r = 0; r < kMaxCluster; r++)
+          if (r < ranks) x += cluster.map_shared_rank(mine, r)[digit];
+      }
+      above += before(x);
+      if (above < need && above + x >= need) {
+        s_found[0] = static_cast<uint32_t>(digit);
+        s_found[1] = above;
+        s_found[2] = x;
+      }
     }
     __syncthreads();
     prefix = (prefix << (pass == 2 ? 10 : 11)) | s_found[0];
     need -= s_found[1];
+    const bool all_of_it = need == s_found[2];   // whatever their lower digits are
     __syncthreads();
+    if (all_of_it) {
+      // keys above `prefix` 0..0 - 1: all of these, and none is left to choose among equals
+      prefix = (pass == 2 ? prefix : prefix << shift) - 1;
+      need = 0;
+      decided = true;
+      break;
+    }
   }
-  if (p.budget == p.sinks + p.recent) prefix = kMustStay - 1;   // nothing else stays
+  if (!decided && need == 0) prefix = kMustStay - 1;            // nothing but what must stay
   // keys above `prefix` stay, of those equal to it the first `need`
   const int per_warp = ((last - first + kWarps - 1) / kWarps + 31) & ~31;
   const int w_first = min(first + warp * per_warp, last), w_last = min(w_first + per_warp, last);
@@ -179,7 +221,7 @@ __global__ void __launch_bounds__(kThreads) select_kernel(const KvEvictParams p)
     for (int w = 0; w < kWarps; w++) sum += s_warp[w][tid];
     s_counts[tid] = sum;
   }
-  cluster.sync();
+  all_sync();
   uint32_t n_above = 0, n_equal = 0;       // before this warp's run
   for (int r = 0; r < rank; r++) {
     const uint32_t* const c = cluster.map_shared_rank(s_counts, r);
@@ -201,59 +243,51 @@ __global__ void __launch_bounds__(kThreads) select_kernel(const KvEvictParams p)
     n_above += __popc(ma);
     n_equal += __popc(me);
   }
-  cluster.sync();                          // no CTA leaves while another still reads its shared memory
+  if (ranks > 1) cluster.sync();           // no CTA leaves while another still reads its shared memory
 }
 
-constexpr int kMoveThreads = 256;
-constexpr int kMoveRows = 16;                               // rows a warp moves
-constexpr int kMoveBlockRows = kMoveRows * kMoveThreads / 32;
+constexpr int kMoveThreads = 128;
+constexpr int kMoveRows = 32;              // rows a block moves
 
 __global__ void __launch_bounds__(kMoveThreads) move_kernel(const KvEvictParams p, int32_t blocks_per_list,
                                                             FastDiv chunk_div) {
-  const int list = blockIdx.x / blocks_per_list;
+  __shared__ const uint8_t* src[2 * kMoveRows];   // keys of row r at 2 r, values at 2 r + 1; nullptr: left out
+  __shared__ uint8_t* dst[2 * kMoveRows];
+  const int list = blockIdx.x / blocks_per_list, j0 = (blockIdx.x - list * blocks_per_list) * kMoveRows;
   const int b = list / p.cache.heads, h = list - b * p.cache.heads;
-  const int lane = threadIdx.x & 31;
-  const int j0 = (blockIdx.x - list * blocks_per_list) * kMoveBlockRows + (threadIdx.x >> 5) * kMoveRows;
   const int count = min(kv_length(p.table, b, nullptr), p.budget);
-  const int rows = min(kMoveRows, count - j0);
-  if (rows <= 0) return;                                    // the whole warp
-  // lanes 0-15 look up the keys of a row, lanes 16-31 its values
-  const bool values = lane >= kMoveRows;
-  const int mine = lane & (kMoveRows - 1);
-  const uint8_t* src = nullptr;
-  uint8_t* dst = nullptr;
-  if (mine < rows) {
-    const int j = j0 + mine;
+  const int rows = min(kMoveRows, count - j0), j = j0 + static_cast<int>(threadIdx.x);
+  int32_t dp = -1, d_slot = 0;
+  if (static_cast<int>(threadIdx.x) < rows) dp = kv_locate(p.cache, p.new_pages, p.new_stride, b, j, &d_slot);
+  asm volatile("griddepcontrol.wait;" ::: "memory");        // every block: this grid never ends before the other
+  if (rows <= 0) return;
+  if (static_cast<int>(threadIdx.x) < rows) {
     const int32_t from = p.kept[static_cast<int64_t>(list) * p.budget + j];
-    int32_t s_slot, d_slot;
+    int32_t s_slot;
     const int32_t sp = kv_locate(p.cache, p.table.pages, p.table.stride, b, from, &s_slot);
-    const int32_t dp = kv_locate(p.cache, p.new_pages, p.new_stride, b, j, &d_slot);
-    if (sp >= 0 && dp >= 0) {
-      const int64_t page = values ? p.cache.v_page : p.cache.k_page, slot = values ? p.cache.v_slot : p.cache.k_slot;
-      uint8_t* const pool = (values ? p.cache.values : p.cache.keys) + h * (values ? p.cache.v_head : p.cache.k_head);
-      src = pool + sp * page + s_slot * slot;
-      dst = pool + dp * page + d_slot * slot;
-      if (!values) p.cache.weights[kv_weight_index(p.cache, dp, h, d_slot)] = p.cache.weights[kv_weight_index(p.cache, sp, h, s_slot)];
-    }
+    const bool ok = sp >= 0 && dp >= 0;
+    src[2 * threadIdx.x] = ok ? p.cache.keys + sp * p.cache.k_page + s_slot * p.cache.k_slot + h * p.cache.k_head : nullptr;
+    src[2 * threadIdx.x + 1] = ok ? p.cache.values + sp * p.cache.v_page + s_slot * p.cache.v_slot + h * p.cache.v_head : nullptr;
+    dst[2 * threadIdx.x] = p.cache.keys + dp * p.cache.k_page + d_slot * p.cache.k_slot + h * p.cache.k_head;
+    dst[2 * threadIdx.x + 1] = p.cache.values + dp * p.cache.v_page + d_slot * p.cache.v_slot + h * p.cache.v_head;
+    if (ok) p.cache.weights[kv_weight_index(p.cache, dp, h, d_slot)] = p.cache.weights[kv_weight_index(p.cache, sp, h, s_slot)];
   }
-  // keys and values of the rows: 2 * rows lines of `chunks` 16-byte pieces, line 2 r + 1 the values of row r
+  __syncthreads();
   const int chunks = p.row_bytes / 16, work = rows * 2 * chunks;
   constexpr int U = 4;
-  for (int w0 = 0; w0 < work; w0 += 32 * U) {
+  for (int w0 = threadIdx.x; w0 < work; w0 += kMoveThreads * U) {
     uint4 x[U];
     uint8_t* to[U];
 #pragma unroll
     for (int u = 0; u < U; u++) {
-      const int w = w0 + u * 32 + lane;
-      const int line = static_cast<int>(fast_div(w, chunk_div)), c = w - line * chunks;
-      const int owner = ((line >> 1) & (kMoveRows - 1)) + (line & 1) * kMoveRows;
-      const uint64_t s = __shfl_sync(0xffffffffu, reinterpret_cast<uint64_t>(src), owner);
-      const uint64_t d = __shfl_sync(0xffffffffu, reinterpret_cast<uint64_t>(dst), owner);
+      const int w = w0 + u * kMoveThreads;
       to[u] = nullptr;
-      if (w < work && s != 0) {
-        x[u] = *reinterpret_cast<const uint4*>(s + c * 16);
-        to[u] = reinterpret_cast<uint8_t*>(d + c * 16);
-      }
+      if (w >= work) continue;
+      const int line = static_cast<int>(fast_div(w, chunk_div)), c = w - line * chunks;
+      const uint8_t* const s = src[line];
+      if (s == nullptr) continue;
+      x[u] = *reinterpret_cast<const uint4*>(s + c * 16);
+      to[u] = dst[line] + c * 16;
     }
 #pragma unroll
     for (int u = 0; u < U; u++)
@@ -261,14 +295,15 @@ __global__ void __launch_bounds__(kMoveThreads) move_kernel(const KvEvictParams 
   }
 }
 
-template <bool CACHED>
+template <bool CACHED, int kThreads>
 void launch_select(const KvEvictParams& p, int ranks, size_t smem, cudaStream_t stream) {
   static std::atomic<uint64_t> done{0};    // one bit per device
   int dev = 0;
   NVE_B200_CUDA(cudaGetDevice(&dev));
   const uint64_t bit = uint64_t{1} << (dev & 63);
+  const auto kernel = select_kernel<CACHED, kThreads>;
   if (CACHED && !(done.load(std::memory_order_acquire) & bit)) {
-    NVE_B200_CUDA(cudaFuncSetAttribute(select_kernel<CACHED>, cudaFuncAttributeMaxDynamicSharedMemorySize, kMaxCached * 4));
+    NVE_B200_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kMaxCached * 4));
     done.fetch_or(bit, std::memory_order_acq_rel);
   }
   cudaLaunchConfig_t cfg{};
@@ -282,7 +317,7 @@ void launch_select(const KvEvictParams& p, int ranks, size_t smem, cudaStream_t 
   attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
   cfg.attrs = &attr;
   cfg.numAttrs = 1;
-  NVE_B200_CUDA(cudaLaunchKernelEx(&cfg, select_kernel<CACHED>, p));
+  NVE_B200_CUDA(cudaLaunchKernelEx(&cfg, kernel, p));
 }
 
 }  // namespace
@@ -292,19 +327,27 @@ void launch_kv_evict(const KvEvictParams& p, int sms, cudaStream_t stream) {
   // CTAs of a cluster: enough for every SM to have work, as long as each still has 2048 rows; more where a run
   // would not fit into shared memory
   int ranks = 1;
-  while (ranks < kMaxCluster && ((lists * ranks < sms && p.table.capacity / ranks >= 4096) ||
+  while (ranks < kMaxCluster && ((lists * ranks * 2 <= sms && p.table.capacity / ranks >= 4096) ||
                                  p.table.capacity / ranks > kMaxCached - 64)) {
     ranks *= 2;
   }
   const int step = ((p.table.capacity + ranks - 1) / ranks + 31) & ~31;
-  if (step <= kMaxCached) launch_select<true>(p, ranks, size_t(step) * 4, stream);
-  else launch_select<false>(p, ranks, 0, stream);
+  if (step <= 4096) launch_select<true, 256>(p, ranks, size_t(step) * 4, stream);
+  else if (step <= kMaxCached) launch_select<true, 1024>(p, ranks, size_t(step) * 4, stream);
+  else launch_select<false, 1024>(p, ranks, 0, stream);
   const int32_t most = std::min(p.budget, p.table.capacity);
   if (most == 0) return;
-  const int32_t per_list = static_cast<int32_t>(ceil_div(most, kMoveBlockRows));
-  move_kernel<<<static_cast<unsigned>(lists * per_list), kMoveThreads, 0, stream>>>(
-      p, per_list, make_fast_div(static_cast<uint32_t>(p.row_bytes / 16)));
-  NVE_B200_CUDA(cudaGetLastError());
+  const int32_t per_list = static_cast<int32_t>(ceil_div(most, kMoveRows));
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3(static_cast<unsigned>(lists * per_list));
+  cfg.blockDim = dim3(kMoveThreads);
+  cfg.stream = stream;
+  cudaLaunchAttribute attr{};
+  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr.val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = &attr;
+  cfg.numAttrs = 1;
+  NVE_B200_CUDA(cudaLaunchKernelEx(&cfg, move_kernel, p, per_list, make_fast_div(static_cast<uint32_t>(p.row_bytes / 16))));
 }
 
 }  // namespace nve_b200
