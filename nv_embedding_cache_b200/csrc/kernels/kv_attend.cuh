@@ -259,6 +259,7 @@ __global__ void __launch_bounds__(kThreads, Shape<ST, DP, WM, NT>::kMinCtas) att
     constexpr int kEach = kOwnRows / 32;
     const int lw = warp - kComputeWarps;
     const int row_chunks = width * static_cast<int>(sizeof(ST)) / 16, q_chunks = width / 8;
+    const int pair_chunks = (row_chunks + 1) & ~1;          // what the products read
     longlong2* const own = offs + lw * kOwnRows;
     // addresses of this lane's rows (keys, values) of the tile `at`; 0: no such row
     auto locate = [&](longlong2 (&o)[kEach]) {
@@ -322,16 +323,24 @@ __global__ void __launch_bounds__(kThreads, Shape<ST, DP, WM, NT>::kMinCtas) att
           }
         }
       } else {
+        // the lane's chunk moves on by 32 chunks of rows of pair_chunks
+        const int r_step = 32 / pair_chunks, c_step = 32 - r_step * pair_chunks;
+        int r = lane / pair_chunks, c = lane - r * pair_chunks;
 #pragma unroll 2
-        for (int x = 0; x < kCopies; x++) {
-          const int r = x * kRowsStep + r_lane;
+        for (int x = 0; x < kOwnRows / 32 * pair_chunks; x++) {
           const longlong2 o = own[r];
-          // chunks behind the row's width and rows that are not there become zeros: a NaN left in a page never meets
-          // the products
-          const bool ok = o.x != 0 && c_lane < row_chunks;
-          const uint32_t dst = k_addr + chunk_at<S::kRowBytes>(r, c_lane);
-          cp_async16(dst, ok ? reinterpret_cast<const uint8_t*>(o.x) + c_lane * 16 : p.cache.keys, ok);
-          cp_async16(dst + S::kTileBytes, ok ? reinterpret_cast<const uint8_t*>(o.y) + c_lane * 16 : p.cache.values, ok);
+          // the chunk that makes the count even, and rows that are not there, become zeros: a NaN left in a page
+          // never meets the products
+          const bool ok = o.x != 0 && c < row_chunks;
+          const uint32_t dst = k_addr + chunk_at<S::kRowBytes>(r, c);
+          cp_async16(dst, ok ? reinterpret_cast<const uint8_t*>(o.x) + c * 16 : p.cache.keys, ok);
+          cp_async16(dst + S::kTileBytes, ok ? reinterpret_cast<const uint8_t*>(o.y) + c * 16 : p.cache.values, ok);
+          r += r_step;
+          c += c_step;
+          if (c >= pair_chunks) {
+            c -= pair_chunks;
+            r++;
+          }
         }
       }
       if (first) {                                          // the unit's queries
@@ -360,6 +369,8 @@ __global__ void __launch_bounds__(kThreads, Shape<ST, DP, WM, NT>::kMinCtas) att
   // ================================ computing warps ================================
   const int wm = warp % WM, wt = warp / WM;                 // heads kHeads wm.., rows kWarpRows wt.. of the tile
   const int row = lane >> 2, col = (lane & 3) * 2;          // of a product's 16 x 8 results: rows row, row + 8, columns col, col + 1
+  // steps of 16 values that hold any: the columns behind them are neither copied nor multiplied
+  const int steps = kE4m3 ? ((width + 31) / 32) * 2 : (width + 15) / 16;
   float acc[kSteps][NT][4];                                 // values x heads
   float m_run[NT][2], l_run[NT][2];                         // of heads col, col + 1; the sum of this lane's rows
   uint32_t qf[kKeepQ ? kSteps : 1][NT][2];
@@ -474,6 +485,7 @@ __global__ void __launch_bounds__(kThreads, Shape<ST, DP, WM, NT>::kMinCtas) att
       if constexpr (!kE4m3) {
 #pragma unroll
         for (int s = 0; s < kSteps; s++) {
+          if (s >= steps) break;
           uint32_t b[NT][2];
           if constexpr (kKeepQ) {
 #pragma unroll
@@ -495,6 +507,7 @@ __global__ void __launch_bounds__(kThreads, Shape<ST, DP, WM, NT>::kMinCtas) att
       } else {
 #pragma unroll
         for (int s = 0; s < kSteps; s += 2) {
+          if (s >= steps) break;
           uint32_t b[2][NT][2];
 #pragma unroll
           for (int u = 0; u < 2; u++) {
@@ -605,7 +618,8 @@ __global__ void __launch_bounds__(kThreads, Shape<ST, DP, WM, NT>::kMinCtas) att
         }
       if constexpr (!kE4m3) {
 #pragma unroll
-        for (int s = 0; s < kSteps; s++)
+        for (int s = 0; s < kSteps; s++) {
+          if (s >= steps) break;
 #pragma unroll
           for (int blk = 0; blk < kBlocks; blk++) {
             uint32_t a[4];    // transposed: values 0-7, 8-15 of rows 0-7, then of rows 8-15
@@ -613,9 +627,11 @@ __global__ void __launch_bounds__(kThreads, Shape<ST, DP, WM, NT>::kMinCtas) att
 #pragma unroll
             for (int n = 0; n < NT; n++) mma16816<kBf16>(acc[s][n], a, b[blk][n][0], b[blk][n][1]);
           }
+        }
       } else {
 #pragma unroll
-        for (int s = 0; s < kSteps; s += 2)
+        for (int s = 0; s < kSteps; s += 2) {
+          if (s >= steps) break;
 #pragma unroll
           for (int blk = 0; blk < kBlocks; blk++) {
             // transposed 16-bit units: a lane gets values 2u, 2u + 1 (u = lane / 4) of two rows, byte by byte; even
@@ -631,6 +647,7 @@ __global__ void __launch_bounds__(kThreads, Shape<ST, DP, WM, NT>::kMinCtas) att
               for (int n = 0; n < NT; n++) mma16816<false>(acc[s + u][n], a, b[blk][n][0], b[blk][n][1]);
             }
           }
+        }
       }
     }
 
