@@ -163,12 +163,13 @@ void append(const nve_b200_kv_cache_t* cache, const nve_b200_kv_append_t* a, cud
   NVE_B200_ARG(a->num_tokens >= 0 && a->num_tokens <= kIntMax, who, ": number of tokens must be in [0, 2^31)");
   p.table = table_of(cache, a->page_table, a->page_table_stride, a->pages_per_sequence, a->lengths, a->num_sequences,
                      -1, who);
-  if (a->num_sequences == 0) {
+  if (a->num_sequences == 0) {              // every token is padding
     NVE_B200_ARG(a->num_tokens == 0 || a->csr_offsets != nullptr, who, ": tokens without a sequence");
-    return;
+    if (a->num_tokens == 0) return;
+  } else {
+    NVE_B200_ARG(a->new_lengths != nullptr, who, ": new_lengths is NULL");
+    NVE_B200_ARG(a->new_lengths != a->lengths, who, ": new_lengths must not be lengths");
   }
-  NVE_B200_ARG(a->new_lengths != nullptr, who, ": new_lengths is NULL");
-  NVE_B200_ARG(a->new_lengths != a->lengths, who, ": new_lengths must not be lengths");
   if (a->csr_offsets == nullptr) {
     NVE_B200_ARG(a->num_tokens % a->num_sequences == 0, who, ": num_tokens is not a multiple of num_sequences");
     p.per_sequence = static_cast<int32_t>(a->num_tokens / a->num_sequences);

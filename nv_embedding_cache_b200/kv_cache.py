@@ -8,9 +8,11 @@ its embedding tables, with the verbs of the embedding cache.
 * :func:`rotary` is the rotation alone, differentiable, for training: positions with one or more axes.
 
 A sequence is a row of ``page_table`` (int32 page ids, entries behind the last row are not read) and a length
-(int32).  Pages are the caller's to hand out and to free.  Tensors live on the cache's device; calls run on the
+(int32).  Pages are the caller's to hand out and to free; sequences may share pages as long as no call writes them
+(append, accumulated weights, the new pages of an eviction).  Tensors live on the cache's device; calls run on the
 current stream of that device, allocate their outputs and scratch from torch, never synchronise, and can be captured
-into CUDA graphs.  Page ids and lengths are checked by the kernels; :meth:`PagedKVCache.check` reports.
+into CUDA graphs.  Page ids and lengths are checked by the kernels; :meth:`PagedKVCache.check` reports.  The cache is
+for serving: its methods have no gradient and refuse tensors that ask for one.
 """
 from __future__ import annotations
 
@@ -258,6 +260,8 @@ class PagedKVCache:
         if t.device != self.device or t.dim() != 3 or t.shape[2] != self.head_width:
             raise ValueError(f"{name} must be [.., heads, {self.head_width}] on {self.device}")
         dtype = t.dtype
+        if t.requires_grad and torch.is_grad_enabled():
+            raise ValueError(f"{name} requires a gradient, which the cache does not give: call under torch.no_grad()")
         if dtype is _E4M3 or (dtype is not self.dtype and (self.dtype is not _E4M3 or dtype not in _DTYPES
                                                            or dtype is torch.float32)):
             raise ValueError(f"{name} must have the cache's type, or fp16 or bf16 for an E4M3 cache")
@@ -274,7 +278,8 @@ class PagedKVCache:
         n = self._table(page_table, lengths)
         dtype = self._row_dtype(k, "k")
         tokens = k.shape[0]
-        if v.dtype is not k.dtype or v.shape != k.shape or v.device != self.device or k.shape[1] != self.num_heads:
+        self._row_dtype(v, "v")
+        if v.dtype is not k.dtype or v.shape != k.shape or k.shape[1] != self.num_heads:
             raise ValueError("k and v must agree and have the cache's heads")
         k, v = _rows(k), _rows(v)
         turned = None

@@ -125,6 +125,24 @@ def test_rotary_gradient_against_differences(torch_cuda):
         assert abs(float((grad.double() * e.double()).sum()) - want) <= tol
 
 
+def test_rotary_second_derivative_and_no_gradient(torch_cuda):
+    """The gradient is linear in the incoming one: its own gradient is the forward rotation."""
+    torch = torch_cuda
+    g = gen(torch, 4)
+    plan, freq, axis = plan_of(torch, 16, 2, True)
+    pos = torch.randint(0, 500, (2, 9), generator=g, device="cuda", dtype=torch.int32)
+    x = torch.randn((9, 3, 32), generator=g, device="cuda", requires_grad=True)
+    up = torch.randn(x.shape, generator=g, device="cuda", requires_grad=True)
+    first, = torch.autograd.grad(kv().rotary(x, None, pos, plan), x, up, create_graph=True)
+    v = torch.randn(x.shape, generator=g, device="cuda")
+    second, = torch.autograd.grad(first, up, v)
+    want, m = turned(torch, v, pos, freq, axis, True)
+    within(second, want, 2.0**-21 * m + rounding(torch, "f32", want), "second")
+    with torch.no_grad():
+        out = kv().rotary(x, up, pos, plan)
+    assert not out[0].requires_grad and torch.equal(out[0], kv().rotary(x, None, pos, plan).detach())
+
+
 def test_rotary_strides_broadcasts_and_single_gradients(torch_cuda):
     torch = torch_cuda
     g = gen(torch, 5)
@@ -564,6 +582,66 @@ def test_append_same_number_each_and_without_rotation(torch_cuda):
         assert torch.equal(raw(torch, x.keys[p, s]), raw(torch, k[b:b + 1])) and torch.equal(raw(torch, x.values[p, s]), raw(torch, -k[b:b + 1]))
     out, n = x.cache.append(k[:0], k[:0], x.table, x.lengths, q=k[:0])
     assert n.tolist() == [4, 0, 9] and out.shape == (0, 2, 64)
+
+
+def test_append_of_padding_alone(torch_cuda):
+    torch = torch_cuda
+    x = Batch(torch, [3], heads=1, width=16, cache="bf16", page=4, room=2, seed=33)
+    old = [t.clone() for t in (x.keys, x.values, x.weights)]
+    k = torch.randn((5, 1, 16), generator=x.g, device="cuda").bfloat16()
+    none = torch.zeros((0, 2), dtype=torch.int32, device="cuda")
+    q, n = x.cache.append(k, k, none, x.lengths[:0], q=k, offsets=torch.zeros(1, dtype=torch.int32, device="cuda"))
+    assert n.shape == (0,) and bool((q == 0).all())
+    q, n = x.cache.append(k, k, x.table, x.lengths, q=k, offsets=torch.tensor([2, 2], dtype=torch.int32, device="cuda"))
+    assert n.tolist() == [3] and bool((q == 0).all())
+    for a, b in zip(old, (x.keys, x.values, x.weights)):
+        assert torch.equal(raw(torch, a), raw(torch, b))
+    # the same through the C ABI without zero_padding: rows of padding are left as they were
+    out = torch.full_like(k, 7.0)
+    r = capi.HeadRows(k.data_ptr(), out.data_ptr(), 32, 32, 32, 32, 1)
+    kv_rows = capi.HeadRows(k.data_ptr(), None, 32, 32, 0, 0, 1)
+    off = torch.tensor([1, 3], dtype=torch.int32, device="cuda")
+    new = torch.zeros(1, dtype=torch.int32, device="cuda")
+    args = capi.KvAppend(capi.DTYPE_BFLOAT16, 5, r, kv_rows, kv_rows, None, x.table.data_ptr(), x.table.stride(0),
+                         x.table.shape[1], 1, x.lengths.data_ptr(), off.data_ptr(), new.data_ptr(), 0)
+    capi.check(capi.lib.nve_b200_kv_append(C.byref(x.cache._view), C.byref(args), None))
+    torch.cuda.synchronize()
+    assert new.tolist() == [5] and torch.equal(out[1:3], k[1:3])
+    assert bool((out[[0, 3, 4]] == 7.0).all())
+
+
+def test_refusals_of_the_python_edge(torch_cuda):
+    torch = torch_cuda
+    x = Batch(torch, [3, 4], heads=2, width=64, cache="bf16", page=4, seed=34, spare=4)
+    q = torch.randn((2, 4, 64), device="cuda").bfloat16()
+    attend = x.cache.attend
+    plan, _, _ = plan_of(torch, 32, 2, False)
+    pos = torch.zeros((2, 2), dtype=torch.int32, device="cuda")
+    k = q[:, :2]
+    for call, word in (
+            (lambda: attend(q.half(), x.table, x.lengths), "cache's type"), (lambda: attend(q[:1], x.table, x.lengths), "one row"),
+            (lambda: attend(q, x.table.long(), x.lengths), "int32"), (lambda: attend(q, x.table, x.lengths.cpu()), "int32"),
+            (lambda: attend(q, x.table, x.lengths[:1]), "one row"), (lambda: attend(q[..., :32], x.table, x.lengths), "64"),
+            (lambda: attend(q.clone().requires_grad_(), x.table, x.lengths), "gradient"),
+            (lambda: x.cache.append(k, k[:1], x.table, x.lengths), "agree"), (lambda: x.cache.append(q, q, x.table, x.lengths), "heads"),
+            (lambda: x.cache.append(k, k, x.table, x.lengths, rotary=plan), "together"),
+            (lambda: x.cache.append(k, k, x.table, x.lengths, rotary=plan, positions=pos.long()), "int32"),
+            (lambda: x.cache.append(k, k, x.table, x.lengths, rotary=plan, positions=pos[:1]), "positions"),
+            (lambda: x.cache.append(k, k, x.table, x.lengths, offsets=pos[0]), "one entry more"),
+            (lambda: x.cache.append(k, k, x.table, x.lengths, q=q[:1]), "tokens"),
+            (lambda: x.cache.evict(x.table, x.lengths, x.table, 0), "budget"), (lambda: x.cache.evict(x.table, x.lengths, x.table[:1], 1), "one row"),
+            (lambda: kv().rotary(q, k.half(), pos, plan), "agree"), (lambda: kv().rotary(q.long(), None, pos, plan), "fp32"),
+            (lambda: kv().PagedKVCache(x.keys, x.values[:1], x.weights), "match"),
+            (lambda: kv().PagedKVCache(x.keys, x.values, x.weights[:1]), "weights"),
+            (lambda: kv().PagedKVCache(x.keys, x.values, key_scale=torch.ones(2, device="cuda")), "E4M3")):
+        with pytest.raises(ValueError, match=word):
+            call()
+    for call in (lambda: attend(q[:, :3], x.table, x.lengths), lambda: attend(q, x.table, x.lengths, max_length=1000),
+                 lambda: x.cache.evict(x.table, x.lengths, x.spare[:0].view(2, 0), 5),
+                 lambda: kv().PagedKVCache(x.keys, x.values).evict(x.table, x.lengths, x.spare[:2].view(2, 1), 2),
+                 lambda: kv().PagedKVCache(x.keys, x.values).attend(q, x.table, x.lengths, accumulate_weights=True)):
+        with pytest.raises(capi.NveError):
+            call()
 
 
 def test_append_saturates_and_keeps_nan_in_e4m3(torch_cuda):
