@@ -42,11 +42,20 @@ constexpr int kLoadWarps = 2;
 constexpr int kThreads = (kComputeWarps + kLoadWarps) * 32;
 constexpr float kNegInf = -__builtin_huge_valf();
 
-__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, bool take) {
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(take ? 16 : 0) : "memory");
+// The cache is read once: its lines are the first to leave L2 again, and the scores, which the join reads, stay (64
+// sequences of 3000 rows: 149 -> 138 us for both launches).
+__device__ __forceinline__ uint64_t read_once() {
+  uint64_t policy;
+  asm("createpolicy.fractional.L2::evict_first.b64 %0, 1.0;" : "=l"(policy));
+  return policy;
 }
-__device__ __forceinline__ void cp_async16_full(uint32_t dst, const void* src) {
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, bool take, uint64_t policy) {
+  asm volatile("cp.async.cg.shared.global.L2::cache_hint [%0], [%1], 16, %2, %3;" ::"r"(dst), "l"(src), "r"(take ? 16 : 0),
+               "l"(policy)
+               : "memory");
+}
+__device__ __forceinline__ void cp_async16_full(uint32_t dst, const void* src, uint64_t policy) {
+  asm volatile("cp.async.cg.shared.global.L2::cache_hint [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "l"(policy) : "memory");
 }
 // The barrier gets this thread's arrival when its copies so far are done.
 __device__ __forceinline__ void cp_async_arrive(uint64_t* bar) {
@@ -260,6 +269,7 @@ __global__ void __launch_bounds__(kThreads, Shape<ST, DP, WM, NT>::kMinCtas) att
     const int lw = warp - kComputeWarps;
     const int row_chunks = width * static_cast<int>(sizeof(ST)) / 16, q_chunks = width / 8;
     const int pair_chunks = (row_chunks + 1) & ~1;          // what the products read
+    const uint64_t policy = read_once();
     longlong2* const own = offs + lw * kOwnRows;
     // addresses of this lane's rows (keys, values) of the tile `at`; 0: no such row
     auto locate = [&](longlong2 (&o)[kEach]) {
@@ -318,8 +328,8 @@ __global__ void __launch_bounds__(kThreads, Shape<ST, DP, WM, NT>::kMinCtas) att
           for (int x = 0; x < kCopies / kPeriod; x++) {
             const longlong2 o = from[x * 8];
             const uint32_t dst = to + x * 8 * S::kRowBytes;
-            cp_async16_full(dst, reinterpret_cast<const uint8_t*>(o.x) + c_lane * 16);
-            cp_async16_full(dst + S::kTileBytes, reinterpret_cast<const uint8_t*>(o.y) + c_lane * 16);
+            cp_async16_full(dst, reinterpret_cast<const uint8_t*>(o.x) + c_lane * 16, policy);
+            cp_async16_full(dst + S::kTileBytes, reinterpret_cast<const uint8_t*>(o.y) + c_lane * 16, policy);
           }
         }
       } else {
@@ -333,8 +343,8 @@ __global__ void __launch_bounds__(kThreads, Shape<ST, DP, WM, NT>::kMinCtas) att
           // never meets the products
           const bool ok = o.x != 0 && c < row_chunks;
           const uint32_t dst = k_addr + chunk_at<S::kRowBytes>(r, c);
-          cp_async16(dst, ok ? reinterpret_cast<const uint8_t*>(o.x) + c * 16 : p.cache.keys, ok);
-          cp_async16(dst + S::kTileBytes, ok ? reinterpret_cast<const uint8_t*>(o.y) + c * 16 : p.cache.values, ok);
+          cp_async16(dst, ok ? reinterpret_cast<const uint8_t*>(o.x) + c * 16 : p.cache.keys, ok, policy);
+          cp_async16(dst + S::kTileBytes, ok ? reinterpret_cast<const uint8_t*>(o.y) + c * 16 : p.cache.values, ok, policy);
           r += r_step;
           c += c_step;
           if (c >= pair_chunks) {
@@ -352,7 +362,7 @@ __global__ void __launch_bounds__(kThreads, Shape<ST, DP, WM, NT>::kMinCtas) att
         for (int id = lw * 32 + lane; id < S::kUnitRows * (DP / 8); id += kLoadWarps * 32) {
           const int r = id / (DP / 8), c = id % (DP / 8);
           const bool ok = r < n && c < q_chunks;
-          cp_async16(q_addr + chunk_at<DP * 2>(r, c), ok ? src + r * p.q_head + c * 16 : p.q, ok);
+          cp_async16(q_addr + chunk_at<DP * 2>(r, c), ok ? src + r * p.q_head + c * 16 : p.q, ok, policy);
         }
       }
       cp_async_arrive(full + stage);
