@@ -3,7 +3,8 @@
 The product is ``libnve_b200.so`` (C ABI declared in ``include/nve_c_api.h`` and
 ``include/nve_b200_ops.h``).  This package holds its sources (``csrc/``), the build recipe
 (``build.py``), a ctypes binding of the C ABI (``capi``), the Python layer classes that mirror the
-reference's pynve bindings (``pynve``) and seeded synthetic workload generators (``datagen``).
+reference's pynve bindings (``pynve``), the paged key/value cache (``kv_cache``) and seeded synthetic workload
+generators (``datagen``).
 There is no CPU fallback: importing ``capi`` without the built library raises.
 """
 

@@ -223,10 +223,13 @@ __global__ void __launch_bounds__(kThreads) select_kernel(const KvEvictParams p)
   }
   all_sync();
   uint32_t n_above = 0, n_equal = 0;       // before this warp's run
-  for (int r = 0; r < rank; r++) {
-    const uint32_t* const c = cluster.map_shared_rank(s_counts, r);
-    n_above += c[0];
-    n_equal += c[1];
+#pragma unroll
+  for (int r = 0; r < kMaxCluster; r++) {
+    if (r < rank) {
+      const uint32_t* const c = cluster.map_shared_rank(s_counts, r);
+      n_above += c[0];
+      n_equal += c[1];
+    }
   }
   for (int w = 0; w < warp; w++) {
     n_above += s_warp[w][0];
