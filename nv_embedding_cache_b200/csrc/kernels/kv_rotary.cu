@@ -159,7 +159,8 @@ __global__ void __launch_bounds__(kThreads, 4) rotary_kernel(const RotaryParams 
     if (two) y = *reinterpret_cast<const V*>(src + gap * static_cast<int64_t>(sizeof(T)));
   };
   set_item();
-  const bool works = t < nt && item < p.items;
+  const int32_t token_lanes = kThreads / p.lanes / p.row_lanes;
+  const bool works = t < min(nt, token_lanes) && item < p.items;   // threads that fill no whole token lane are idle
   if (works) load(t, r, a, b);
 
   if constexpr (TO_CACHE) {
@@ -242,7 +243,6 @@ __global__ void __launch_bounds__(kThreads, 4) rotary_kernel(const RotaryParams 
   };
 
   if (works) {
-    const int32_t token_lanes = kThreads / p.lanes / p.row_lanes;
     float2 cs[kPairs];
     int32_t cs_token = -1, cs_item = -1;
     for (;;) {

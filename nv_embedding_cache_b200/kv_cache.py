@@ -27,6 +27,7 @@ _E4M3 = torch.float8_e4m3fn
 _DTYPES = {torch.float32: capi.DTYPE_FLOAT32, torch.float16: capi.DTYPE_FLOAT16, torch.bfloat16: capi.DTYPE_BFLOAT16,
            _E4M3: capi.DTYPE_E4M3}
 _INT32 = torch.int32
+_INT32_MAX = 0x7fffffff
 _raw_stream = torch._C._cuda_getCurrentRawStream
 _current_device = torch._C._cuda_getDevice
 _GROUPS = (None, capi.HeadRows * 1, capi.HeadRows * 2)
@@ -256,6 +257,14 @@ class PagedKVCache:
             raise ValueError("page_table and lengths must have one row per sequence")
         return n
 
+    def _most_rows(self, pages: int, max_length: int | None) -> int:
+        rows = pages * self.page_size
+        if max_length is None:
+            max_length = rows
+        if not 0 <= max_length <= rows or rows > _INT32_MAX:
+            raise ValueError(f"max_length must be in [0, {rows}], the rows of the page table, which must be below 2^31")
+        return max_length
+
     def _row_dtype(self, t: torch.Tensor, name: str) -> int:
         if t.device != self.device or t.dim() != 3 or t.shape[2] != self.head_width:
             raise ValueError(f"{name} must be [.., heads, {self.head_width}] on {self.device}")
@@ -319,8 +328,7 @@ class PagedKVCache:
             raise ValueError("q must have one row per sequence")
         heads, width, device = q.shape[1], self.head_width, self.device
         pages = page_table.shape[1]
-        if max_length is None:
-            max_length = pages * self.page_size
+        max_length = self._most_rows(pages, max_length)
         q = _rows(q)
         e = q.element_size()
         s = q.stride()
@@ -357,11 +365,10 @@ class PagedKVCache:
         _int32(new_page_table, self.device, 2, "new_page_table")
         if new_page_table.shape[0] != n:
             raise ValueError("new_page_table must have one row per sequence")
-        if budget <= 0:
-            raise ValueError("budget must be positive")
+        if not 0 < budget <= _INT32_MAX or sinks < 0 or recent < 0 or sinks + recent > budget:
+            raise ValueError("budget must be positive and hold sinks + recent rows")
         pages = page_table.shape[1]
-        if max_length is None:
-            max_length = pages * self.page_size
+        max_length = self._most_rows(pages, max_length)
         kept = torch.empty((n, self.num_heads, budget), dtype=_INT32, device=self.device)
         new_lengths = torch.empty_like(lengths, memory_format=torch.contiguous_format)
         args = capi.KvEvict(n, page_table.data_ptr(), page_table.stride(0), pages, lengths.data_ptr(), max_length,

@@ -192,6 +192,22 @@ def test_rotary_in_place_and_zero_tokens(torch_cuda):
     assert kv().rotary(x[:0], x[:0], pos[:, :0], plan)[0].shape == (0, 3, 40)
 
 
+@pytest.mark.parametrize("tokens,heads,width,pairs", [(40000, 6, 80, 40), (40000, 1, 24, 4), (30011, 7, 40, 20)])
+def test_rotary_in_place_turns_every_row_once(torch_cuda, tokens, heads, width, pairs):
+    """Many tokens of rows whose items do not divide a block's threads, turned where they are."""
+    torch = torch_cuda
+    g = gen(torch, 9)
+    plan, freq, axis = plan_of(torch, pairs, 1, False)
+    x = torch.randn((tokens, heads, width), generator=g, device="cuda", dtype=torch.float16)
+    pos = torch.randint(0, 999, (1, tokens), generator=g, device="cuda", dtype=torch.int32)
+    want = kv().rotary(x, None, pos, plan)
+    args = plan._args(pos, tokens, x.device)
+    r = capi.HeadRows(x.data_ptr(), x.data_ptr(), heads * width * 2, width * 2, heads * width * 2, width * 2, heads)
+    capi.check(capi.lib.nve_b200_rotary(C.byref(args), capi.DTYPE_FLOAT16, width, tokens, C.byref(r), 1, 0, None))
+    torch.cuda.synchronize()
+    assert torch.equal(x, want)
+
+
 # ---- a cache and a batch -------------------------------------------------------------------------
 class Batch:
     """A cache whose free memory is NaN (E4M3: its NaN), and sequences with shuffled pages; -1 behind the last page."""
@@ -629,14 +645,16 @@ def test_refusals_of_the_python_edge(torch_cuda):
             (lambda: x.cache.append(k, k, x.table, x.lengths, rotary=plan, positions=pos[:1]), "positions"),
             (lambda: x.cache.append(k, k, x.table, x.lengths, offsets=pos[0]), "one entry more"),
             (lambda: x.cache.append(k, k, x.table, x.lengths, q=q[:1]), "tokens"),
-            (lambda: x.cache.evict(x.table, x.lengths, x.table, 0), "budget"), (lambda: x.cache.evict(x.table, x.lengths, x.table[:1], 1), "one row"),
+            (lambda: x.cache.evict(x.table, x.lengths, x.table, 0), "budget"), (lambda: x.cache.evict(x.table, x.lengths, x.table, 4, sinks=3, recent=2), "sinks"),
+            (lambda: x.cache.evict(x.table, x.lengths, x.table, 1 << 32), "budget"), (lambda: attend(q, x.table, x.lengths, max_length=1000), "max_length"),
+            (lambda: attend(q, x.table, x.lengths, max_length=1 << 32), "max_length"), (lambda: attend(q, x.table, x.lengths, max_length=-1), "max_length"), (lambda: x.cache.evict(x.table, x.lengths, x.table[:1], 1), "one row"),
             (lambda: kv().rotary(q, k.half(), pos, plan), "agree"), (lambda: kv().rotary(q.long(), None, pos, plan), "fp32"),
             (lambda: kv().PagedKVCache(x.keys, x.values[:1], x.weights), "match"),
             (lambda: kv().PagedKVCache(x.keys, x.values, x.weights[:1]), "weights"),
             (lambda: kv().PagedKVCache(x.keys, x.values, key_scale=torch.ones(2, device="cuda")), "E4M3")):
         with pytest.raises(ValueError, match=word):
             call()
-    for call in (lambda: attend(q[:, :3], x.table, x.lengths), lambda: attend(q, x.table, x.lengths, max_length=1000),
+    for call in (lambda: attend(q[:, :3], x.table, x.lengths),
                  lambda: x.cache.evict(x.table, x.lengths, x.spare[:0].view(2, 0), 5),
                  lambda: kv().PagedKVCache(x.keys, x.values).evict(x.table, x.lengths, x.spare[:2].view(2, 1), 2),
                  lambda: kv().PagedKVCache(x.keys, x.values).attend(q, x.table, x.lengths, accumulate_weights=True)):
