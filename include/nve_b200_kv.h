@@ -45,7 +45,7 @@ typedef struct {
   int64_t key_strides[3];    /* bytes: page, slot, head; multiples of 16, any order in memory */
   int64_t value_strides[3];
   float* weights;            /* [num_pages][num_heads][page_size] dense: attention each row drew; NULL = not kept */
-  const float* key_scale;    /* E4M3 rows, [num_heads]: value = scale * stored; NULL = 1 */
+  const float* key_scale;    /* E4M3 rows, [num_heads]: value = scale * stored, positive and not subnormal; NULL = 1 */
   const float* value_scale;
   nve_data_type_t dtype;     /* FLOAT16, BFLOAT16 or E4M3 */
   int64_t num_pages;

@@ -104,7 +104,7 @@ __device__ __forceinline__ TokenPlace place_token(const RotaryParams& p, int32_t
     first = b * p.per_sequence;
   }
   r.padding = false;
-  const int64_t row = static_cast<int64_t>(kv_length(p.table, b, p.cache.status)) + (t - first);
+  const int64_t row = static_cast<int64_t>(kv_length(p.table, b, p.cache.status)) + t - first;
   if (row < 0 || row >= p.table.capacity) {
     kv_flag(p.cache.status, NVE_B200_KV_BAD_LENGTH);
     return r;
@@ -165,8 +165,8 @@ __global__ void __launch_bounds__(kThreads, 4) rotary_kernel(const RotaryParams 
 
   if constexpr (TO_CACHE) {
     for (int32_t s = blockIdx.x * kThreads + threadIdx.x; s < p.table.sequences; s += gridDim.x * kThreads) {
-      const int32_t more = p.offsets != nullptr ? __ldg(p.offsets + s + 1) - __ldg(p.offsets + s) : p.per_sequence;
-      const int64_t n = static_cast<int64_t>(kv_length(p.table, s, p.cache.status)) + max(more, 0);
+      const int64_t more = p.offsets != nullptr ? static_cast<int64_t>(__ldg(p.offsets + s + 1)) - __ldg(p.offsets + s) : p.per_sequence;
+      const int64_t n = kv_length(p.table, s, p.cache.status) + max(more, int64_t{0});
       p.new_lengths[s] = static_cast<int32_t>(min(n, static_cast<int64_t>(p.table.capacity)));
     }
     for (int32_t i = threadIdx.x >> 5; i < nt; i += kThreads / 32) {
