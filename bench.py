@@ -90,7 +90,12 @@ def run_reference_arm(args):
     if rank != 0:
         return
     from nv_embedding_cache_b200 import datagen as dg
+    from oracle import build as oracle_build
     from oracle.pyoracle import Reference
+    if oracle_build.build_reference() is None:
+        print(json.dumps({"impl": "reference", "unavailable": "neither the reference checkout nor its prebuilt CPU library is on this machine"}),
+              flush=True)
+        return
     perm = dg.permutation(NUM_ROWS)
     table = dg.normal_table(NUM_ROWS, WIDTH, 0.02, 20, np.float16)
     batches = [make_batch(0, b, 0, perm) for b in range(NUM_BATCHES)]

@@ -29,6 +29,8 @@ HERE = Path(__file__).resolve().parent
 OUT = HERE / "_ref"
 # the reference checkout: NVE_REFERENCE_DIR, else a directory named "reference" beside this repository
 REFERENCE = Path(os.environ.get("NVE_REFERENCE_DIR", str(HERE.parents[1] / "reference")))
+if REFERENCE.is_dir() and not any(REFERENCE.iterdir()):     # an empty directory is no checkout
+    REFERENCE = REFERENCE / "absent"
 
 REF_SOURCES = [
     "host_embedding_layer", "linear_host_table", "host_table", "host_table_detail", "table",
