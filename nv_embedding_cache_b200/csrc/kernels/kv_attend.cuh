@@ -32,6 +32,7 @@
 #include "../common.hpp"
 #include "bulk_copy.cuh"
 #include "kv_attend.hpp"
+#include "kv_launch.cuh"
 
 namespace nve_b200 {
 
@@ -191,6 +192,7 @@ __global__ void __launch_bounds__(kThreads, Shape<ST, DP, WM, NT>::kMinCtas) att
       mbar_init(empty + s, kComputeWarps);
     }
   }
+  grid_wait();
   // ---- the number of tiles, and where this CTA's run of them begins
   __shared__ int32_t s_sum[kThreads / 32];
   __shared__ int32_t s_start[3];
@@ -259,8 +261,7 @@ __global__ void __launch_bounds__(kThreads, Shape<ST, DP, WM, NT>::kMinCtas) att
   int stage = 0;
   uint32_t phase = 0;                                       // of the stage's barriers
 
-  // the join may be scheduled from here on; it waits for this grid's end before it reads what is written here
-  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  grid_release();                                           // the join reads what this grid writes after its wait only
 
   if (warp >= kComputeWarps) {
     // ================================ loading warps ================================
@@ -774,8 +775,7 @@ struct Launcher {
   }
   static void launch(const KvAttendParams& p, cudaStream_t stream) {
     prepare();
-    attend_kernel<ST, DP, WM, NT><<<p.ctas, kThreads, Shape<ST, DP, WM, NT>::kSmem, stream>>>(p);
-    NVE_B200_CUDA(cudaGetLastError());
+    launch_overlapped(attend_kernel<ST, DP, WM, NT>, p.ctas, kThreads, Shape<ST, DP, WM, NT>::kSmem, 1, stream, p);
   }
 };
 

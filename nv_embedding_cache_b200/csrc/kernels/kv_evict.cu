@@ -13,8 +13,7 @@
 // Small blocks, many per SM: a block looks its rows up, a thread each, and copies them with four 16-byte pieces of a
 // thread in flight.  Warps that do both for themselves, or look the next rows up while they copy, keep fewer loads in
 // flight and took 60 and 69 us where this takes 48 (32 lists of 8192 rows of 256 bytes: 5.6 TB/s).
-// The launch overlaps the end of the choosing one (programmatic dependent launch): new pages are looked up before the
-// wait.
+// New pages are looked up before the wait for the choosing launch.
 #include <algorithm>
 #include <atomic>
 
@@ -22,6 +21,7 @@
 
 #include "../common.hpp"
 #include "kv_evict.hpp"
+#include "kv_launch.cuh"
 
 namespace nve_b200 {
 
@@ -58,7 +58,8 @@ __global__ void __launch_bounds__(kThreads) select_kernel(const KvEvictParams p)
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int list = blockIdx.x / ranks;     // (sequence, head)
   const int b = list / p.cache.heads, h = list - b * p.cache.heads;
-  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  grid_wait();
+  grid_release();
   const int length = kv_length(p.table, b, p.cache.status);
   const int count = min(length, p.budget);
   int32_t* const kept = p.kept + static_cast<int64_t>(list) * p.budget;
@@ -262,7 +263,8 @@ __global__ void __launch_bounds__(kMoveThreads) move_kernel(const KvEvictParams 
   const int rows = min(kMoveRows, count - j0), j = j0 + static_cast<int>(threadIdx.x);
   int32_t dp = -1, d_slot = 0;
   if (static_cast<int>(threadIdx.x) < rows) dp = kv_locate(p.cache, p.new_pages, p.new_stride, b, j, &d_slot);
-  asm volatile("griddepcontrol.wait;" ::: "memory");        // every block: this grid never ends before the other
+  grid_wait();
+  grid_release();
   if (rows <= 0) return;
   if (static_cast<int>(threadIdx.x) < rows) {
     const int32_t from = p.kept[static_cast<int64_t>(list) * p.budget + j];
@@ -309,18 +311,8 @@ void launch_select(const KvEvictParams& p, int ranks, size_t smem, cudaStream_t 
     NVE_B200_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kMaxCached * 4));
     done.fetch_or(bit, std::memory_order_acq_rel);
   }
-  cudaLaunchConfig_t cfg{};
-  cfg.gridDim = dim3(static_cast<unsigned>(p.table.sequences * p.cache.heads * ranks));
-  cfg.blockDim = dim3(kThreads);
-  cfg.dynamicSmemBytes = smem;
-  cfg.stream = stream;
-  cudaLaunchAttribute attr{};
-  attr.id = cudaLaunchAttributeClusterDimension;
-  attr.val.clusterDim.x = static_cast<unsigned>(ranks);
-  attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
-  cfg.attrs = &attr;
-  cfg.numAttrs = 1;
-  NVE_B200_CUDA(cudaLaunchKernelEx(&cfg, kernel, p));
+  launch_overlapped(kernel, static_cast<int64_t>(p.table.sequences) * p.cache.heads * ranks, kThreads, smem,
+                    static_cast<unsigned>(ranks), stream, p);
 }
 
 }  // namespace
@@ -341,16 +333,8 @@ void launch_kv_evict(const KvEvictParams& p, int sms, cudaStream_t stream) {
   const int32_t most = std::min(p.budget, p.table.capacity);
   if (most == 0) return;
   const int32_t per_list = static_cast<int32_t>(ceil_div(most, kMoveRows));
-  cudaLaunchConfig_t cfg{};
-  cfg.gridDim = dim3(static_cast<unsigned>(lists * per_list));
-  cfg.blockDim = dim3(kMoveThreads);
-  cfg.stream = stream;
-  cudaLaunchAttribute attr{};
-  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr.val.programmaticStreamSerializationAllowed = 1;
-  cfg.attrs = &attr;
-  cfg.numAttrs = 1;
-  NVE_B200_CUDA(cudaLaunchKernelEx(&cfg, move_kernel, p, per_list, make_fast_div(static_cast<uint32_t>(p.row_bytes / 16))));
+  launch_overlapped(move_kernel, lists * per_list, kMoveThreads, 0, 1, stream, p, per_list,
+                    make_fast_div(static_cast<uint32_t>(p.row_bytes / 16)));
 }
 
 }  // namespace nve_b200

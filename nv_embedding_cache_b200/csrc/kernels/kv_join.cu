@@ -11,12 +11,12 @@
 // heads on bf16 rows of 128); read as the first to leave it, so that what does not fit costs no more than itself (131 MB
 // of scores: 34 -> 29 us).  What a block does before its first score (tiles before its sequence, the lse of its
 // heads) is a chain of waits, so slices are as long as filling the GPU allows.
-// The launch overlaps the first one's end (programmatic dependent launch): what needs only the lengths is done before
-// the wait.
+// What needs only the lengths is done before the wait for the first launch.
 #include <algorithm>
 
 #include "../common.hpp"
 #include "kv_attend.hpp"
+#include "kv_launch.cuh"
 
 namespace nve_b200 {
 
@@ -58,8 +58,10 @@ __device__ __forceinline__ float2 join_ml(float2 a, float2 b) {
   return make_float2(m, a.y * exp2f(a.x - base) + b.y * exp2f(b.x - base));
 }
 
-// Waits for the end of the first launch.  Every block does, so that this grid never ends before that one.
-__device__ __forceinline__ void first_launch_done() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+__device__ __forceinline__ void first_launch_done() {
+  grid_wait();
+  grid_release();
+}
 
 struct JoinPlan {
   int32_t weight_blocks;             // the first blocks: slices of rows
@@ -288,16 +290,8 @@ void launch_kv_join(const KvAttendParams& p, int sms, cudaStream_t stream) {
   plan.heads = 1;
   while (plan.heads < kWarps && plan.heads < p.chunk && unit_count * ceil_div(p.chunk, plan.heads) > sms) plan.heads *= 2;
   plan.per_unit = static_cast<int32_t>(ceil_div(p.chunk, plan.heads));
-  cudaLaunchConfig_t cfg{};
-  cfg.gridDim = dim3(static_cast<unsigned>(plan.weight_blocks + unit_count * plan.per_unit));
-  cfg.blockDim = dim3(kThreads);
-  cfg.stream = stream;
-  cudaLaunchAttribute attr{};
-  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr.val.programmaticStreamSerializationAllowed = 1;
-  cfg.attrs = &attr;
-  cfg.numAttrs = 1;
-  NVE_B200_CUDA(cudaLaunchKernelEx(&cfg, p.chunk <= 4 ? join_kernel<4> : join_kernel<8>, p, plan));
+  launch_overlapped(p.chunk <= 4 ? join_kernel<4> : join_kernel<8>, plan.weight_blocks + unit_count * plan.per_unit, kThreads,
+                    0, 1, stream, p, plan);
 }
 
 int kv_attend_resident(nve_data_type_t cache_dtype, int width, int rows_per_unit) {

@@ -13,6 +13,7 @@
 #include <algorithm>
 
 #include "../common.hpp"
+#include "kv_launch.cuh"
 #include "kv_rotary.cuh"
 
 namespace nve_b200 {
@@ -159,6 +160,8 @@ __global__ void __launch_bounds__(kThreads, 4) rotary_kernel(const RotaryParams 
     if (two) y = *reinterpret_cast<const V*>(src + gap * static_cast<int64_t>(sizeof(T)));
   };
   set_item();
+  grid_wait();
+  grid_release();
   const int32_t token_lanes = kThreads / p.lanes / p.row_lanes;
   const bool works = t < min(nt, token_lanes) && item < p.items;   // threads that fill no whole token lane are idle
   if (works) load(t, r, a, b);
@@ -291,10 +294,9 @@ __global__ void __launch_bounds__(kThreads, 4) rotary_kernel(const RotaryParams 
 
 template <typename T, int VEC, bool INTERLEAVED, bool TO_CACHE, bool E4M3>
 void launch_one(const RotaryParams& p, cudaStream_t stream) {
-  const int64_t token_blocks = ceil_div(p.tokens, p.tokens_per_block);
-  const unsigned grid = static_cast<unsigned>(std::max<int64_t>(token_blocks, 1));
-  rotary_kernel<T, VEC, INTERLEAVED, TO_CACHE, E4M3>
-      <<<grid, kThreads, size_t(p.tokens_per_block) * p.pairs * sizeof(float2), stream>>>(p);
+  launch_overlapped(rotary_kernel<T, VEC, INTERLEAVED, TO_CACHE, E4M3>,
+                    std::max<int64_t>(1, ceil_div(p.tokens, p.tokens_per_block)), kThreads,
+                    size_t(p.tokens_per_block) * p.pairs * sizeof(float2), 1, stream, p);
 }
 
 template <typename T, int VEC, bool INTERLEAVED>
@@ -338,7 +340,6 @@ void launch_type(RotaryParams& p, bool e4m3, bool interleaved, int sms, cudaStre
     if (interleaved) launch_dest<T, 1, true>(p, e4m3, stream);
     else launch_dest<T, 1, false>(p, e4m3, stream);
   }
-  NVE_B200_CUDA(cudaGetLastError());
 }
 
 }  // namespace
