@@ -793,6 +793,122 @@ def test_evict_reports_bad_pages_and_leaves_their_rows_out(torch_cuda):
         assert bool(same.all())
 
 
+# ---- order on the stream -------------------------------------------------------------------------
+def test_calls_follow_what_is_before_them_on_the_stream(torch_cuda):
+    """Launches may overlap the end of what runs before them; what they read has to be complete all the same: lengths made
+    by a host copy, a fill, another stream or the call before, eager and captured."""
+    torch = torch_cuda
+    x = Batch(torch, [4000, 4000], heads=4, width=128, cache="bf16", page=16, seed=60, room=200)
+    q = torch.randn((2, 8, 128), generator=x.g, device="cuda").bfloat16()
+    ends = [torch.tensor(e, dtype=torch.int32, device="cuda") for e in ([4000, 77], [5, 3999])]
+    want = [x.cache.attend(q, x.table, e) for e in ends]
+    pinned = ends[0].cpu().pin_memory()
+    n = torch.zeros(2, dtype=torch.int32, device="cuda")
+
+    def steps(first):
+        first()
+        a = x.cache.attend(q, x.table, n)
+        n.zero_()
+        z = x.cache.attend(q, x.table, n)
+        n.copy_(ends[1])
+        return a, z, x.cache.attend(q, x.table, n)
+
+    def right(a, z, b):
+        return torch.equal(a, want[0]) and bool((z == 0).all()) and torch.equal(b, want[1])
+
+    torch.cuda.synchronize()
+    got = [steps(lambda: n.copy_(pinned, non_blocking=True)) for _ in range(50)]
+    torch.cuda.synchronize()
+    assert all(right(*g) for g in got)
+    side = torch.cuda.Stream()
+
+    def other_stream():
+        main = torch.cuda.current_stream()
+        side.wait_stream(main)
+        with torch.cuda.stream(side):
+            n.copy_(ends[0])
+        main.wait_stream(side)
+
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = steps(other_stream)
+    for _ in range(20):
+        for o in out:
+            o.fill_(3)
+        graph.replay()
+    torch.cuda.synchronize()
+    assert right(*out)
+    k = torch.randn((2, 4, 128), generator=x.g, device="cuda").bfloat16()
+    runs = []
+    for _ in range(5):
+        m, outs = x.lengths, []
+        for s in range(30):
+            _, m = x.cache.append(k * ((s + 1) / 30), k, x.table, m)
+            outs.append(x.cache.attend(q, x.table, m))
+        runs.append(torch.stack(outs))
+    torch.cuda.synchronize()
+    assert m.tolist() == [4030, 4030] and all(torch.equal(runs[0], r) for r in runs)
+    x.cache.check()
+
+
+def test_threads_share_a_cache(torch_cuda):
+    """Two host threads, a stream each, the same cache: reads do not disturb one another."""
+    import threading
+    torch = torch_cuda
+    x = Batch(torch, [3000, 500], heads=2, width=128, cache="f16", page=16, seed=61)
+    qs = [torch.randn((2, h, 128), generator=x.g, device="cuda").half() for h in (4, 16)]
+    want = [x.cache.attend(q, x.table, x.lengths) for q in qs]
+    torch.cuda.synchronize()
+    wrong = []
+
+    def work(i):
+        stream = torch.cuda.Stream()
+        with torch.cuda.stream(stream):
+            outs = [x.cache.attend(qs[i], x.table, x.lengths) for _ in range(100)]
+        stream.synchronize()
+        if not all(torch.equal(o, want[i]) for o in outs):
+            wrong.append(i)
+
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not wrong
+
+
+def test_rotary_backward_in_a_graph(torch_cuda):
+    """Forward and gradient captured and replayed on new values.  (No eager graph of the same leaf may be alive then: torch
+    keeps the leaf's node on the stream of that one, and refuses the capture for any function.)"""
+    torch = torch_cuda
+    g = gen(torch, 62)
+    plan, freq, axis = plan_of(torch, 32, 2, False)
+    pos = torch.randint(0, 500, (2, 50), generator=g, device="cuda", dtype=torch.int32)
+    x = torch.randn((50, 4, 64), generator=g, device="cuda", requires_grad=True)
+    up = torch.randn(x.shape, generator=g, device="cuda")
+
+    def eager():
+        out = kv().rotary(x, None, pos, plan)
+        return out.detach(), torch.autograd.grad(out, x, up)[0]
+
+    first = eager()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = kv().rotary(x, None, pos, plan)
+        grad, = torch.autograd.grad(out, x, up)
+        out = out.detach()
+    graph.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(out, first[0]) and torch.equal(grad, first[1])
+    with torch.no_grad():
+        x.mul_(-0.5)
+    up.copy_(torch.randn(x.shape, generator=g, device="cuda"))
+    graph.replay()
+    torch.cuda.synchronize()
+    again = eager()
+    assert torch.equal(out, again[0]) and torch.equal(grad, again[1])
+
+
 # ---- together ------------------------------------------------------------------------------------
 @pytest.mark.parametrize("cache", ["bf16", "e4m3"])
 def test_a_decode_run_with_eviction(torch_cuda, cache):
