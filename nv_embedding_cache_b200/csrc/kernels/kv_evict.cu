@@ -133,10 +133,9 @@ __global__ void __launch_bounds__(kThreads) select_kernel(const KvEvictParams p)
       }
     }
     __syncthreads();
+#pragma unroll 4
     for (int c = warp; c < 64; c += kWarps) {
-      uint32_t x = mine[c * 32 + lane];
-#pragma unroll
-      for (int o = 16; o > 0; o >>= 1) x += __shfl_xor_sync(0xffffffffu, x, o);
+      const uint32_t x = __reduce_add_sync(0xffffffffu, mine[c * 32 + lane]);
       if (lane == 0) coarse[pass & 1][c] = x;
     }
     all_sync();
