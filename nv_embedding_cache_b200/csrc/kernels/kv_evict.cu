@@ -5,10 +5,10 @@
 // the largest of all) and stay in shared memory; a radix select over digits of 11, 11 and 10 bits finds the key of
 // the last row that stays: every CTA counts the digits of its run, and after one cluster barrier a digit a warp of
 // every CTA finds it for itself from all CTAs' counts, read over DSMEM: first among 64 sums of 32 digits, then among
-// those 32 (reading all 2048 counts of eight CTAs instead: 33 us against 21 for 32 lists of 26 000 rows).  Then ballots become places in ascending
-// order.  No sort, no scratch in memory, the weights are read once: 4 bytes per row and head.  Latency bounds
-// it (a chain of page lookup, weights, three rounds of counting, places): 10 us for 128 lists of 1000 rows, 24 us for 4
-// of 131 071.
+// those 32 (reading all 2048 counts of eight CTAs instead: 33 us against 21 for 32 lists of 26 000 rows).  Then ballots
+// become places in ascending order.  No sort, no scratch in memory, the weights are read once: 4 bytes per row and head.
+// Latency bounds it (a chain of page lookup, weights, three rounds of counting, places): 10 us for 128 lists of 1000
+// rows, 24 us for 4 of 131 071.
 //
 // Moving: rows of 2 width values per kept row and head, read from anywhere, written page after page; HBM bounds it.
 // Small blocks, many per SM: a block looks its rows up, a thread each, and copies them with four 16-byte pieces of a

@@ -6,6 +6,8 @@
 // A thread then keeps those of one item (a 16-byte vector of the row, or two for the split pairing: the vector of
 // the a's and that of the b's) in registers and walks over the rows of several heads, the next row's load always under
 // way; the first one's starts before the angles.  The queries, keys and values of a token go through one launch.
+// Held at 64 registers, four blocks per SM: 65 us for 16 384 tokens of 40 heads of 128 in bf16 (5.2 TB/s; three blocks 69,
+// five, which spill, 97), 73 us for the append of 13 391 tokens of 48 heads into E4M3 rows (4.1 TB/s).
 //
 // The angle is the product of a 32-bit integer and an fp32 number: exact in 64 bits up to its last two bits.  It is
 // reduced there (in turns, so that the reduction is a subtraction of an integer) and only the remainder is
